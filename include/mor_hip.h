@@ -54,6 +54,8 @@ extern "C" {
 #define MOR_FMT_E5M2 1
 #define MOR_FMT_E3M2 2
 #define MOR_FMT_E2M3 3
+/* 4-bit codes: the MX wire format and its product only */
+#define MOR_FMT_E2M1 4
 /* mor_block_format only: no quantization.  The kernel that would quantize blocks of this shape reads every block,
  * finds its amax and writes the block back unchanged: what the memory system gives that kernel's access pattern
  * (a measurement aid; blocks of one row and up to 2048 elements go through the general block kernels for it). */
@@ -197,6 +199,11 @@ MOR_API int mor_selftest_hw_cast(uint64_t* mismatches, void* stream);
  */
 MOR_API int mor_selftest_hw_wire(uint64_t* mismatches, void* stream);
 
+/* The same for the scaled E2M1 converts: mismatches[0], the codes of every finite bf16 value with every
+ * scale exponent in [-126, 126]; mismatches[1], the value of every code with every exponent the decode
+ * uses the convert for (device pointer, 2 x uint64). */
+MOR_API int mor_selftest_hw_fp4(uint64_t* mismatches, void* stream);
+
 /*
  * The MX wire format as operands of the gfx950 scaled matrix instruction (no counterpart in the
  * reference): out [16, 16] fp32 = A x B^T for two [16, 128] tensors given as mor_mx_quantize gives
@@ -221,6 +228,10 @@ MOR_API int mor_selftest_mx_mfma(const void* payload_a, const void* scales_a, co
  * return with MOR_FLAG_TORCH_EMULATION for 1 x 32 blocks and sf_type 2.  A zero block has scale
  * byte 127.  FP8 payload: one byte per element (OCP E4M3 / E5M2 encodings).  FP6 payload (E2M3 /
  * E3M2): 32 codes packed little-endian into 24 bytes, element i in bits [6i, 6i + 6) of its block.
+ * E2M1 payload (by the same rule; no bf16 op has it): two codes to a byte, 16 bytes a block, element
+ * i in bits [4i, 4i + 4).  Inputs are finite in the 6-bit formats; in the 8-bit ones a NaN or an
+ * infinity has a NaN code; E2M1 has neither: a block with one gets scale byte 255 (the E8M0 NaN) and
+ * zero codes, and decodes to 32 NaNs.
  * cols must be a multiple of 32; tensors and payloads 16-byte aligned, scales 4-byte aligned.
  */
 MOR_API size_t mor_mx_payload_bytes(int64_t rows, int64_t cols, int fmt);
@@ -236,9 +247,56 @@ MOR_API int mor_mx_quantize(const void* input, void* payload, void* scales, int6
 MOR_API int mor_mx_quantize_dual(const void* input, void* row_payload, void* row_scales, void* col_payload,
                          void* col_scales, int64_t rows, int64_t cols, int fmt, void* stream);
 
+/* mor_mx_quantize_dual for any number of rows and for two formats: the last block of every column is filled
+ * up with zeros, so that col_payload is [cols, ceil(rows / 32) * 32 * bits / 8] and col_scales
+ * [cols, ceil(rows / 32)].  Formats (row_fmt, col_fmt): (E4M3, E4M3), (E5M2, E5M2), (E2M1, E2M1), and
+ * (E2M1, E4M3) for a layer that multiplies in 4 bits and keeps its activation in 8. */
+MOR_API int mor_mx_quantize_dual_ragged(const void* input, void* row_payload, void* row_scales, void* col_payload,
+                         void* col_scales, int64_t rows, int64_t cols, int row_fmt, int col_fmt, void* stream);
+
 /* payload + scales -> bf16 [rows, cols] (blocks of 32 along rows). */
 MOR_API int mor_mx_dequantize(const void* payload, const void* scales, void* output, int64_t rows,
                       int64_t cols, int fmt, void* stream);
+
+/*
+ * The product of two tensors in the MX wire format (no counterpart in the reference, whose callers
+ * multiply the dequantized bf16 tensors): output [m, n] bf16 = A x B^T for A [m, k] and B [n, k] as
+ * mor_mx_quantize gives them, formats E4M3, E5M2 and E2M1 in any pair,
+ *   output[i, j] = bf16(sum over t of value(A[i, t]) * value(B[j, t]))
+ * summed in fp32 by the scaled matrix instructions of gfx950 straight from codes and scale bytes, and
+ * rounded to nearest even once.  The instructions align the products of one step to the largest of them:
+ * 4-bit products lose nothing by that, the others the low bits of small ones (some 1e-5 of the sum of
+ * magnitudes).  A NaN code or a scale byte of 255 makes its row or column NaN.
+ * k a positive multiple of 32 below 2^23; m and n positive, below 2^31; payloads 16-byte, output 2-byte
+ * aligned.  Every result depends on the operands and the shape alone (no atomics).
+ * The workspace (mor_mx_matmul_workspace_bytes, 0 for most shapes) holds fp32 partial sums of products
+ * with few rows and columns, whose k is split; 16-byte aligned, not shared by calls that overlap.
+ */
+MOR_API size_t mor_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt);
+MOR_API int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_fmt, const void* b_payload,
+                          const void* b_scales, int b_fmt, void* output, int64_t m, int64_t n, int64_t k,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gated activation that keeps its inputs in 8 bits (no counterpart in the reference):
+ *   output = bf16(gate * sigmoid(gate) * up), computed in fp32,
+ * and for the backward pass the E4M3 codes and scale bytes of gate and up (the rule above; blocks of 32
+ * along rows, the last block of a row filled up with zeros): codes [rows, ceil(cols / 32) * 32] bytes,
+ * scales [rows, ceil(cols / 32)] bytes, 2.0625 instead of 4 bytes per element.  A block with an infinity
+ * or a NaN has scale byte 255 and comes back as NaNs.
+ * gate and up: rows of cols contiguous elements, gate_stride / up_stride elements from row to row
+ * (>= cols; the halves of one projection); output contiguous.  All four code and scale pointers NULL:
+ * nothing is kept.  codes 8-byte, bf16 tensors 2-byte aligned; rows * ceil(cols / 32) < 2^30.
+ */
+MOR_API int mor_swiglu_mx(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, void* output,
+                          void* gate_codes, void* gate_scales, void* up_codes, void* up_scales,
+                          int64_t rows, int64_t cols, void* stream);
+/* The gradients from grad (bf16 [rows, cols], contiguous) and what mor_swiglu_mx kept; with g and u the
+ * decoded values and s = sigmoid(g): grad_gate = bf16(grad * u * s * (1 + g * (1 - s))), grad_up =
+ * bf16(grad * g * s). */
+MOR_API int mor_swiglu_mx_backward(const void* grad, const void* gate_codes, const void* gate_scales, const void* up_codes,
+                                   const void* up_scales, void* grad_gate, void* grad_up, int64_t rows, int64_t cols,
+                                   void* stream);
 
 /*
  * Fake quantization of a tensor and of its transpose from one read (no counterpart in the

@@ -13,6 +13,7 @@ FLAG_TORCH_EMULATION = 1
 FLAG_SOFTWARE_CAST = 2
 FLAG_REFERENCE_ORDER_SUMS = 4
 FMT_E4M3, FMT_E5M2, FMT_E3M2, FMT_E2M3 = 0, 1, 2, 3
+FMT_E2M1 = 4           # the MX wire format and its product only
 FMT_COPY = -1          # mor_block_format only: the block kernels' access pattern without the arithmetic
 OP_FAKE_QUANTIZE, OP_BLOCK_SCALING, OP_CHANNEL_SCALING, OP_E8MX = 0, 1, 2, 3
 
@@ -35,10 +36,16 @@ SIGNATURES = {
     "mor_mor_stats": (_int, [_vp, _i64, _i64, _i64, _i64, _f64, _i64, _i64, _vp, _u32, _vp]),
     "mor_selftest_hw_cast": (_int, [_vp, _vp]),
     "mor_selftest_hw_wire": (_int, [_vp, _vp]),
+    "mor_selftest_hw_fp4": (_int, [_vp, _vp]),
     "mor_selftest_mx_mfma": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _vp]),
     "mor_mx_payload_bytes": (_sz, [_i64, _i64, _int]),
     "mor_mx_quantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "mor_mx_quantize_dual": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
+    "mor_mx_quantize_dual_ragged": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
+    "mor_mx_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
+    "mor_mx_matmul": (_int, [_vp, _vp, _int, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "mor_swiglu_mx": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "mor_swiglu_mx_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "mor_mx_dequantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "mor_fake_quantize_dual": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "mor_fake_quantize_dual_tiles": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f64, _i64, _i64, _vp]),

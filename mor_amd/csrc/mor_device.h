@@ -13,7 +13,7 @@
 
 namespace mor {
 
-enum : int { FMT_E4M3 = 0, FMT_E5M2 = 1, FMT_E3M2 = 2, FMT_E2M3 = 3 };
+enum : int { FMT_E4M3 = 0, FMT_E5M2 = 1, FMT_E3M2 = 2, FMT_E2M3 = 3, FMT_E2M1 = 4 };      // FMT_E2M1: the wire format only
 
 __device__ __forceinline__ float u2f(uint32_t u) { return __uint_as_float(u); }
 __device__ __forceinline__ uint32_t f2u(float f) { return __float_as_uint(f); }
@@ -23,6 +23,7 @@ template <> struct Fmt<FMT_E4M3> { static constexpr float fmax = 448.0f;   stati
 template <> struct Fmt<FMT_E5M2> { static constexpr float fmax = 57344.0f; static constexpr int mbits = 2; static constexpr int emin = -14; static constexpr bool hw = true; };
 template <> struct Fmt<FMT_E3M2> { static constexpr float fmax = 28.0f;    static constexpr int mbits = 2; static constexpr int emin = -2;  static constexpr bool hw = false; };
 template <> struct Fmt<FMT_E2M3> { static constexpr float fmax = 7.5f;     static constexpr int mbits = 3; static constexpr int emin = 0;   static constexpr bool hw = false; };
+template <> struct Fmt<FMT_E2M1> { static constexpr float fmax = 6.0f;     static constexpr int mbits = 1; static constexpr int emin = 0;   static constexpr bool hw = false; };
 
 __host__ __device__ __forceinline__ float fmax_of(int fmt) {
     return fmt == FMT_E4M3 ? 448.0f : fmt == FMT_E5M2 ? 57344.0f : fmt == FMT_E3M2 ? 28.0f : 7.5f;
@@ -249,7 +250,7 @@ __device__ __forceinline__ Scale make_scale(float s) {
 // use e8); `fast` additionally requires a normal amax.
 template <int F> __device__ __forceinline__ Scale make_scale_e8(float amax) {
     constexpr int eb = (F == FMT_E4M3) ? 8 : (F == FMT_E5M2) ? 15 : (F == FMT_E3M2) ? 4 : 2;
-    constexpr uint32_t mth = (F == FMT_E2M3) ? 0x70u : 0x60u;       // mantissa field of 1.875 / 1.75
+    constexpr uint32_t mth = (F == FMT_E2M3) ? 0x70u : (F == FMT_E2M1) ? 0x40u : 0x60u;       // mantissa field of 1.875 / 1.5 / 1.75
     const uint32_t b = f2u(amax);
     const int ea = (int)(b >> 23);
     Scale sc;

@@ -4,7 +4,7 @@
 // changed scales), for lane l = 16 g + r and row r:
 //   8-bit codes: the 16 codes of columns 16 g .. 16 g + 15 and the 16 codes of columns 64 + 16 g ..., as the two
 //                halves of the lane's 8 registers;
-//   6-bit codes: the 32 codes of columns 32 g .. 32 g + 31, 24 bytes packed as the wire format packs them;
+//   6-bit and 4-bit codes: the 32 codes of columns 32 g .. 32 g + 31, 24 or 16 bytes packed as the wire format packs them;
 //   the scale of the 32 columns 32 b .. 32 b + 31 of row r is taken from lane 16 b + r.
 // All of these are plain loads from the wire format: half an MX block twice or a whole one, and one E8M0 byte.
 // A test of the format, not a GEMM.
@@ -21,7 +21,7 @@ namespace mor {
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// HWF: the instruction's format code (0 E4M3, 1 E5M2, 2 E2M3, 3 E3M2); BYTES per block of 32 codes (32 or 24)
+// HWF: the instruction's format code (0 E4M3, 1 E5M2, 2 E2M3, 3 E3M2, 4 E2M1); BYTES per block of 32 codes (32, 24 or 16)
 template <int HWF, int BYTES>
 __global__ __launch_bounds__(64) void k_mx_mfma_16x16x128(const uint8_t* pa, const uint8_t* sa, const uint8_t* pb,
                                                           const uint8_t* sb, float* out) {
@@ -38,9 +38,9 @@ __global__ __launch_bounds__(64) void k_mx_mfma_16x16x128(const uint8_t* pa, con
             b[4 + i] = (int)*reinterpret_cast<const uint32_t*>(pb + second + 4 * i);
         }
     } else {
-        const int at = (r * 4 + g) * 24;
+        const int at = (r * 4 + g) * BYTES;
 #pragma unroll
-        for (int i = 0; i < 6; ++i) {
+        for (int i = 0; i < BYTES / 4; ++i) {
             a[i] = (int)*reinterpret_cast<const uint32_t*>(pa + at + 4 * i);
             b[i] = (int)*reinterpret_cast<const uint32_t*>(pb + at + 4 * i);
         }
@@ -72,6 +72,7 @@ extern "C" int mor_selftest_mx_mfma(const void* payload_a, const void* scales_a,
         case MOR_FMT_E5M2: k_mx_mfma_16x16x128<1, 32><<<1, 64, 0, st>>>(pa, sa, pb, sb, out); break;
         case MOR_FMT_E2M3: k_mx_mfma_16x16x128<2, 24><<<1, 64, 0, st>>>(pa, sa, pb, sb, out); break;
         case MOR_FMT_E3M2: k_mx_mfma_16x16x128<3, 24><<<1, 64, 0, st>>>(pa, sa, pb, sb, out); break;
+        case MOR_FMT_E2M1: k_mx_mfma_16x16x128<4, 16><<<1, 64, 0, st>>>(pa, sa, pb, sb, out); break;
         default: return mor_fail(MOR_ERR_INVALID_ARGUMENT, "unknown format %d", fmt);
     }
     return mor_check_launch("k_mx_mfma_16x16x128");

@@ -9,8 +9,9 @@
 //                    along columns through an LDS copy of the tile, written transposed ([cols, rows] payload) so that
 //                    the reduction dimension of a weight-gradient GEMM is contiguous
 //   k_mx_dequantize  payload + scales -> bf16
-// All codes come from the gfx950 FP8 converts (E2M3 / E3M2 share the mantissa width of E4M3 / E5M2, see code_pair);
-// FP6 codes are packed little-endian, 32 codes in 24 bytes.  The file also holds k_fq_dual, the fake-quantized
+// FP8 and FP6 codes come from the gfx950 FP8 converts (E2M3 / E3M2 share the mantissa width of E4M3 / E5M2, see
+// code_pair), E2M1 codes from its scaled FP4 convert.  FP6 codes are packed little-endian, 32 codes in 24 bytes, E2M1
+// codes two to a byte, 16 bytes a block.  The file also holds k_fq_dual, the fake-quantized
 // tensor and the fake-quantized transpose from one read.
 
 #include <hip/hip_runtime.h>
@@ -27,12 +28,55 @@ constexpr int WWG = 256;
 
 // Exponent of the block scale, limited to the finite E8M0 range.  The integer form needs a normal amax; the
 // division covers subnormal amax and the far ends of the exponent range.
+// E2M1 has no code for an infinity or a NaN: a block that holds one (amax as block_amax gives it) gets E8_NONFINITE,
+// whose scale byte 127 - e8 is the E8M0 NaN, and decodes to NaNs.
+constexpr int E8_NONFINITE = -128;
 template <int F> __device__ __forceinline__ int wire_e8(float amax) {
+    if constexpr (F == FMT_E2M1) { if (f2u(amax) >= 0x7F800000u) return E8_NONFINITE; }
     if (!(amax > 0.0f)) return 0;
     const Scale sc = make_scale_e8<F>(amax);
     int e8 = sc.e8;
     if (!sc.fast) e8 = (int)((f2u(Fmt<F>::fmax / amax) >> 23) & 0xFF) - 127;
     return min(max(e8, -127), 127);
+}
+
+// The byte of two E2M1 codes of a packed word.  v_cvt_scalef32_pk_fp4_bf16 divides by its scale and rounds to nearest
+// even (mor_selftest_hw_fp4 compares the two forms for every finite bf16 value and every e8 in [-126, 126]); the
+// software form counts the midpoints below |x| * 2^e8, a midpoint itself going to the even code.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ bool fp4_hw_ok(int e8) { return e8 >= -126 && e8 <= 126; }
+__device__ __forceinline__ uint32_t fp4_mag_code(float a) {
+    return (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
+}
+__device__ __forceinline__ uint32_t fp4_pair_sw(uint32_t w, int e8) {
+    if (e8 == E8_NONFINITE) return 0;
+    const uint32_t a = fp4_mag_code(ldexpf(fabsf(bf16_lo(w)), e8)), b = fp4_mag_code(ldexpf(fabsf(bf16_hi(w)), e8));
+    return a | ((w >> 12) & 8u) | ((b | ((w >> 28) & 8u)) << 4);
+}
+// the 8 codes of four packed words, element i in bits [4 i, 4 i + 4)
+__device__ __forceinline__ uint32_t fp4_octet(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int e8) {
+    if (fp4_hw_ok(e8)) {
+        const float scale = u2f((uint32_t)(127 - e8) << 23);
+        uint32_t p = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(bf16x2, w0), scale, 0);
+        p = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(p, __builtin_bit_cast(bf16x2, w1), scale, 1);
+        p = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(p, __builtin_bit_cast(bf16x2, w2), scale, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(p, __builtin_bit_cast(bf16x2, w3), scale, 3);
+    }
+    return fp4_pair_sw(w0, e8) | (fp4_pair_sw(w1, e8) << 8) | (fp4_pair_sw(w2, e8) << 16) | (fp4_pair_sw(w3, e8) << 24);
+}
+// value of an E2M1 code
+__device__ __forceinline__ float fp4_value(uint32_t code) {
+    const uint32_t e = (code >> 1) & 3u, m = code & 1u;
+    const float mag = e == 0 ? 0.5f * (float)m : u2f(((e + 126u) << 23) | (m << 22));
+    return u2f(f2u(mag) | ((code & 8u) << 28));
+}
+// the 8 values of an octet of codes times 2^de, as bf16
+__device__ __forceinline__ uint4 fp4_octet_decode_hw(uint32_t q, int de) {
+    const float scale = u2f((uint32_t)(127 + de) << 23);
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 0)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 2)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3)));
 }
 
 // codes of the two elements of a packed word, in bits 0..bits-1 and bits..2*bits-1 (FP6: fp6_mag_codes).
@@ -55,7 +99,6 @@ template <int F> __device__ __forceinline__ uint64_t code_chunk(uint4 v, int e8)
            ((uint64_t)code_pair<F>(v.z, e8) << (2 * pb)) | ((uint64_t)code_pair<F>(v.w, e8) << (3 * pb));
 }
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 template <int F, bool HIGH> __device__ __forceinline__ uint32_t fp8_pair_decode_hw(uint32_t codes, float scale) {
     if constexpr (F == FMT_E4M3) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)codes, scale, HIGH));
     else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)codes, scale, HIGH));
@@ -85,15 +128,42 @@ __device__ __forceinline__ float chunk_amax(uint4 v) {
     return amax;
 }
 
+// Largest magnitude of the block whose four chunks the lanes of a quad hold.  E2M1: of the bit patterns, so that an
+// infinity or a NaN wins (the other formats carry them in their codes, and a NaN does not take part).
+template <int F> __device__ __forceinline__ float block_amax(uint4 v) {
+    if constexpr (F == FMT_E2M1) {
+        uint32_t m = 0;
+        acc_amax_pk(m, v.x); acc_amax_pk(m, v.y); acc_amax_pk(m, v.z); acc_amax_pk(m, v.w);
+        return u2f(group_umax(amax_bits_of(m), 4));
+    } else return group_max_t<4>(chunk_amax(v), 4);
+}
+// the same of 32 values in one lane
+template <int F> __device__ __forceinline__ float words_amax(const uint32_t (&w)[16]) {
+    if constexpr (F == FMT_E2M1) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc_amax_pk(m, w[i]);
+        return u2f(amax_bits_of(m));
+    } else {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc_amax(amax, w[i]);
+        return amax;
+    }
+}
+
 // Quantizes and stores one chunk; `c` is the chunk's index in the payload's own row-major order (4 chunks = 1 block,
 // held by the 4 lanes of a quad; every lane of the quad must call this).
-// FP8: 8 bytes per lane.  FP6: the quad's 16 words are broadcast to its lanes (DPP), every lane converts the whole
+// FP8: 8 bytes per lane.  E2M1: 4 bytes per lane.  FP6: the quad's 16 words are broadcast to its lanes (DPP), every lane converts the whole
 // block with one instruction and lanes 0..2 store 8 of the 24 bytes each; outside the range of the block convert the
 // software codes are merged across the quad instead.
 template <int F> __device__ __forceinline__ void emit_chunk(uint8_t* payload, int64_t c, uint4 v, int e8, bool ok) {
     if constexpr (Fmt<F>::hw) {
         const uint64_t codes = code_chunk<F>(v, e8);
         if (ok) *reinterpret_cast<uint2*>(payload + c * 8) = make_uint2((uint32_t)codes, (uint32_t)(codes >> 32));
+    } else if constexpr (F == FMT_E2M1) {
+        const uint32_t codes = fp4_octet(v.x, v.y, v.z, v.w, e8);
+        if (ok) *reinterpret_cast<uint32_t*>(payload + c * 4) = codes;
     } else {
         const int j = (int)(c & 3);
         uint32_t lo, hi;
@@ -131,8 +201,7 @@ __global__ __launch_bounds__(WWG) void k_mx_quantize(const uint4* in, uint8_t* p
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int64_t c = base + k * WWG;
-        const float amax = group_max_t<4>(chunk_amax(v[k]), 4);
-        const int e8 = wire_e8<F>(amax);
+        const int e8 = wire_e8<F>(block_amax<F>(v[k]));
         emit_chunk<F>(payload, c, v[k], e8, c < nchunks);
         // the scale bytes of 4 consecutive blocks (16 lanes) leave as one 32-bit store
         const uint32_t sb = (uint32_t)(127 - e8);
@@ -146,7 +215,8 @@ __global__ __launch_bounds__(WWG) void k_mx_quantize(const uint4* in, uint8_t* p
 }
 
 // ------------------------------------------------------------------------------------------------
-// both orientations from one read.  Tile TR rows x 128 columns (TR = 64 or 128); rows % 32 == 0, cols % 32 == 0.
+// both orientations from one read, blocks along rows in format FR, along columns in FC.  Tile TR rows x 128 columns (TR = 64
+// or 128); cols % 32 == 0.  Where rows % 32 != 0 the last block of every column is filled up with zeros.
 constexpr int TILE_C = 128;
 constexpr int TILE_ROWS = 128;
 constexpr int DUAL_THREADS = 512;
@@ -186,15 +256,15 @@ static int dual_tile_map(int64_t tiles_x, int64_t tiles_y) {
     return 0;
 }
 
-template <int F, int TR, int DT>
+template <int FR, int FC, int TR, int DT>
 __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_payload, uint8_t* row_scales,
                                                  uint8_t* col_payload, uint8_t* col_scales, int64_t rows, int64_t cols, int map_mode) {
     constexpr int PITCH = TILE_C + 8;             // bf16 elements per LDS row; keeps the row starts 16-byte aligned
     constexpr int NV = TR * (TILE_C / 8) / DT;   // 16-byte chunks per thread
     constexpr int RB = TR / 32;                   // row blocks per tile column
     constexpr int BPT = TILE_C * RB / DT;        // column blocks per thread
-    constexpr int blk_bytes = 32 * Wire<F>::bits / 8;
-    constexpr int SEG = Fmt<F>::hw ? 16 : 8;      // bytes per lane of the column stores (both divide blk_bytes)
+    constexpr int blk_bytes = 32 * Wire<FC>::bits / 8;
+    constexpr int SEG = blk_bytes % 16 == 0 ? 16 : 8;      // bytes per lane of the column stores (both divide blk_bytes)
     constexpr int CODE_PITCH = (RB * blk_bytes + 16 + 15) / 16 * 16;   // bytes per column of the code tile (padded, 16-byte aligned)
     constexpr int SEGS = RB * blk_bytes / SEG;    // per column
     // one buffer, two uses: the bf16 tile, then the codes of the column blocks (smaller)
@@ -240,15 +310,14 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
     // that everything streams anyway and plain stores are faster.  6-bit codes keep plain stores: a tile's part of
     // a column is 96 bytes, three quarters of a memory line, and streamed parts reach memory before the neighbouring
     // tile's part joins them (8192^2: 49.4 us streamed, 47.3 plain; 16384 x 14336: 265 against 201 us).
-    const bool nt = Wire<F>::bits == 8 && streams_out(rows * cols) && rows * cols <= ((int64_t)128 << 20);
+    const bool nt = Wire<FC>::bits == 8 && streams_out(rows * cols) && rows * cols <= ((int64_t)128 << 20);
     const bool dword_row_scales = (cols & 127) == 0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int ch = k * DT + tid, r = ch >> 4, cc = ch & 15;
-        const float amax = group_max_t<4>(chunk_amax(v[k]), 4);
-        const int e8 = wire_e8<F>(amax);
+        const int e8 = wire_e8<FR>(block_amax<FR>(v[k]));
         const int64_t cidx = (R0 + r) * row_chunks + (C0 >> 3) + cc;       // chunk index in the row-major payload
-        emit_chunk<F>(row_payload, cidx, v[k], e8, ok[k]);
+        emit_chunk<FR>(row_payload, cidx, v[k], e8, ok[k]);
         const uint32_t sb = (uint32_t)(127 - e8);
         const uint32_t s4 = sb | (__shfl_down(sb, 4, 16) << 8) | (__shfl_down(sb, 8, 16) << 16) | (__shfl_down(sb, 12, 16) << 24);
         if (dword_row_scales && cols_valid == TILE_C) {
@@ -260,20 +329,22 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
 #pragma unroll
     for (int h = 0; h < BPT; ++h) {
         const int rb = (tid >> 7) * BPT + h;
-        float amax = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc_amax(amax, w[h][i]);
-        const int e8 = wire_e8<F>(amax);
+        const int e8 = wire_e8<FC>(words_amax<FC>(w[h]));
         s_cscale[c * 4 + rb] = (uint8_t)(127 - e8);
         uint8_t* dst = codes + c * CODE_PITCH + rb * blk_bytes;
-        if constexpr (Fmt<F>::hw) {
+        if constexpr (Fmt<FC>::hw) {
             uint32_t q[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = code_pair<F>(w[h][2 * i], e8) | (code_pair<F>(w[h][2 * i + 1], e8) << 16);
+            for (int i = 0; i < 8; ++i) q[i] = code_pair<FC>(w[h][2 * i], e8) | (code_pair<FC>(w[h][2 * i + 1], e8) << 16);
             *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
             *reinterpret_cast<uint4*>(dst + 16) = make_uint4(q[4], q[5], q[6], q[7]);
+        } else if constexpr (FC == FMT_E2M1) {
+            uint32_t q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = fp4_octet(w[h][4 * i], w[h][4 * i + 1], w[h][4 * i + 2], w[h][4 * i + 3], e8);
+            *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
         } else {
-            const u32x6 d = fp6_hw_ok(e8) ? fp6_block_hw<F>(w[h], e8) : fp6_block_sw<F>(w[h], e8);
+            const u32x6 d = fp6_hw_ok(e8) ? fp6_block_hw<FC>(w[h], e8) : fp6_block_sw<FC>(w[h], e8);
             *reinterpret_cast<uint2*>(dst) = make_uint2(d[0], d[1]);
             *reinterpret_cast<uint2*>(dst + 8) = make_uint2(d[2], d[3]);
             *reinterpret_cast<uint2*>(dst + 16) = make_uint2(d[4], d[5]);
@@ -282,8 +353,8 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
     __syncthreads();
 
     // the transposed payload: a column of the tile is RB * blk_bytes contiguous bytes, SEGS lanes store one column
-    const int64_t col_row_bytes = rows / 32 * blk_bytes;                 // bytes per column in the transposed payload
-    const int valid_bytes = rows_valid / 32 * blk_bytes;
+    const int64_t col_row_bytes = (rows + 31) / 32 * blk_bytes;                 // bytes per column in the transposed payload
+    const int valid_bytes = (rows_valid + 31) / 32 * blk_bytes;
     if (SEG == 16 || ((col_row_bytes & 15) == 0 && rows_valid == TR)) {      // 16 bytes per lane wherever they are aligned
         constexpr int S16 = RB * blk_bytes / 16;
 #pragma unroll
@@ -305,11 +376,11 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
     // scale bytes of the column blocks: RB per column and tile
     if (tid < TILE_C && c < cols_valid) {
         const uint32_t sall = *reinterpret_cast<const uint32_t*>(&s_cscale[c * 4]);
-        uint8_t* dst = col_scales + (C0 + c) * (rows / 32) + R0 / 32;
+        uint8_t* dst = col_scales + (C0 + c) * ((rows + 31) / 32) + R0 / 32;
         if (RB == 4 && (rows & 127) == 0) *reinterpret_cast<uint32_t*>(dst) = sall;
         else if (RB == 2 && (rows & 63) == 0) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)sall;
         else
-            for (int b = 0; b < rows_valid / 32; ++b) dst[b] = (uint8_t)(sall >> (8 * b));
+            for (int b = 0; b < (rows_valid + 31) / 32; ++b) dst[b] = (uint8_t)(sall >> (8 * b));
     }
 }
 
@@ -460,6 +531,14 @@ __global__ __launch_bounds__(WWG) void k_mx_dequantize(const uint8_t* payload, c
             }
             x[0] = hw_unpack<F, 0>(q.x); x[1] = hw_unpack<F, 1>(q.x); x[2] = hw_unpack<F, 2>(q.x); x[3] = hw_unpack<F, 3>(q.x);
             x[4] = hw_unpack<F, 0>(q.y); x[5] = hw_unpack<F, 1>(q.y); x[6] = hw_unpack<F, 2>(q.y); x[7] = hw_unpack<F, 3>(q.y);
+        } else if constexpr (F == FMT_E2M1) {
+            const uint32_t q = *reinterpret_cast<const uint32_t*>(payload + c * 4);
+            if (fp6_decode_hw_ok(de)) {          // v_cvt_scalef32_pk_bf16_fp4
+                store16_rt(out + c, fp4_octet_decode_hw(q, de), streams_out(nchunks * 8));
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = de == 128 ? u2f(0x7FC00000u) : fp4_value(q >> (4 * i));      // 128: the E8M0 NaN
         } else {
             if (fp6_decode_hw_ok(de)) {
                 // every lane of the quad reads its block's 24 bytes (same addresses: one fetch) and decodes all 32 codes
@@ -563,6 +642,34 @@ __global__ __launch_bounds__(WWG) void k_selftest_hw_fp8_decode(unsigned long lo
     if (bad) atomicAdd(mismatches + F, (unsigned long long)bad);
 }
 
+// E2M1 converts: mismatches[0], every bf16 pair of patterns x every scale exponent the hardware convert is used with;
+// mismatches[1], the 16 codes (two octets) x every scale exponent of the decode.
+__global__ __launch_bounds__(WWG) void k_selftest_hw_fp4(unsigned long long* mismatches) {
+    const uint32_t idx = blockIdx.x * WWG + threadIdx.x;
+    if (idx >= 8192u * 253u) return;
+    const int e8 = (int)(idx >> 13) - 126;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = (idx & 8191u) * 8u + 2u * i;
+        w[i] = (lo & 0x7F80u) == 0x7F80u ? 0u : lo | ((lo + 1u) << 16);          // Inf / NaN blocks never reach the convert
+    }
+    const uint32_t want = fp4_pair_sw(w[0], e8) | (fp4_pair_sw(w[1], e8) << 8) | (fp4_pair_sw(w[2], e8) << 16) | (fp4_pair_sw(w[3], e8) << 24);
+    if (fp4_octet(w[0], w[1], w[2], w[3], e8) != want) atomicAdd(mismatches, 1ull);
+}
+__global__ __launch_bounds__(WWG) void k_selftest_hw_fp4_decode(unsigned long long* mismatches) {
+    const int idx = blockIdx.x * WWG + threadIdx.x;
+    if (idx >= 2 * 201) return;
+    const int de = (idx >> 1) - 100;
+    const uint32_t q = (idx & 1) ? 0xFEDCBA98u : 0x76543210u;
+    const uint4 got = fp4_octet_decode_hw(q, de);
+    const uint32_t r[4] = {got.x, got.y, got.z, got.w};
+    unsigned bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad += r[i] != store_pair<true>(ldexpf(fp4_value(q >> (8 * i)), de), ldexpf(fp4_value(q >> (8 * i + 4)), de));
+    if (bad) atomicAdd(mismatches + 1, (unsigned long long)bad);
+}
+
 }  // namespace mor
 
 using namespace mor;
@@ -572,7 +679,7 @@ static int validate_wire(const void* a, const void* b, const void* c, int64_t ro
     if (rows <= 0 || cols <= 0) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "rows and cols must be positive (got %lld x %lld)", (long long)rows, (long long)cols);
     if (cols % 32 || rows % row_multiple)
         return mor_fail(MOR_ERR_INVALID_ARGUMENT, "MX blocks need cols %% 32 == 0 and rows %% %lld == 0 (got %lld x %lld)", (long long)row_multiple, (long long)rows, (long long)cols);
-    if (fmt < MOR_FMT_E4M3 || fmt > MOR_FMT_E2M3) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "unknown element format %d", fmt);
+    if (fmt < MOR_FMT_E4M3 || fmt > MOR_FMT_E2M1) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "unknown element format %d", fmt);
     if (rows > MOR_MAX_ELEMENTS / cols) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "tensor too large (more than 2^35 elements)");
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "tensor and payload must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(c) & 3u) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "scales must be 4-byte aligned");
@@ -581,7 +688,7 @@ static int validate_wire(const void* a, const void* b, const void* c, int64_t ro
 
 extern "C" size_t mor_mx_payload_bytes(int64_t rows, int64_t cols, int fmt) {
     if (rows <= 0 || cols <= 0) return 0;
-    return (size_t)rows * (size_t)cols * ((fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E5M2) ? 8 : 6) / 8;
+    return (size_t)rows * (size_t)cols * ((fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E5M2) ? 8 : fmt == MOR_FMT_E2M1 ? 4 : 6) / 8;
 }
 
 extern "C" int mor_mx_quantize(const void* input, void* payload, void* scales, int64_t rows, int64_t cols, int fmt, void* stream) {
@@ -596,10 +703,22 @@ extern "C" int mor_mx_quantize(const void* input, void* payload, void* scales, i
     switch (fmt) {
         case MOR_FMT_E4M3: k_mx_quantize<FMT_E4M3, NV><<<grid, WWG, 0, st>>>(in, p, s, nchunks); break;
         case MOR_FMT_E5M2: k_mx_quantize<FMT_E5M2, NV><<<grid, WWG, 0, st>>>(in, p, s, nchunks); break;
+        case MOR_FMT_E2M1: k_mx_quantize<FMT_E2M1, NV><<<grid, WWG, 0, st>>>(in, p, s, nchunks); break;
         case MOR_FMT_E3M2: k_mx_quantize<FMT_E3M2, NV><<<grid, WWG, 0, st>>>(in, p, s, nchunks); break;
         default: k_mx_quantize<FMT_E2M3, NV><<<grid, WWG, 0, st>>>(in, p, s, nchunks); break;
     }
     return mor_check_launch("k_mx_quantize");
+}
+
+template <int FR, int FC>
+static int launch_dual(const void* input, void* row_payload, void* row_scales, void* col_payload, void* col_scales, int64_t rows,
+                       int64_t cols, hipStream_t st) {
+    const int64_t tiles_y = (rows + TILE_ROWS - 1) / TILE_ROWS, tiles_x = (cols + TILE_C - 1) / TILE_C;
+    if (tiles_y * tiles_x > 0x7FFFFFFFll) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "too many tiles");
+    k_mx_dual<FR, FC, TILE_ROWS, DUAL_THREADS><<<(unsigned)(tiles_y * tiles_x), DUAL_THREADS, 0, st>>>(
+        static_cast<const uint4*>(input), static_cast<uint8_t*>(row_payload), static_cast<uint8_t*>(row_scales),
+        static_cast<uint8_t*>(col_payload), static_cast<uint8_t*>(col_scales), rows, cols, dual_tile_map(tiles_x, tiles_y));
+    return mor_check_launch("k_mx_dual");
 }
 
 extern "C" int mor_mx_quantize_dual(const void* input, void* row_payload, void* row_scales, void* col_payload, void* col_scales,
@@ -607,19 +726,25 @@ extern "C" int mor_mx_quantize_dual(const void* input, void* row_payload, void* 
     if (int rc = validate_wire(input, row_payload, row_scales, rows, cols, fmt, 32)) return rc;
     if (int rc = validate_wire(input, col_payload, col_scales, rows, cols, fmt, 32)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t tiles = ((rows + TILE_ROWS - 1) / TILE_ROWS) * ((cols + TILE_C - 1) / TILE_C);
-    if (tiles > 0x7FFFFFFFll) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "too many tiles");
-    const uint4* in = static_cast<const uint4*>(input);
-    uint8_t *rp = static_cast<uint8_t*>(row_payload), *rs = static_cast<uint8_t*>(row_scales);
-    uint8_t *cp = static_cast<uint8_t*>(col_payload), *cs = static_cast<uint8_t*>(col_scales);
-    const int mm = dual_tile_map((cols + TILE_C - 1) / TILE_C, (rows + TILE_ROWS - 1) / TILE_ROWS);
     switch (fmt) {
-        case MOR_FMT_E4M3: k_mx_dual<FMT_E4M3, TILE_ROWS, DUAL_THREADS><<<(unsigned)tiles, DUAL_THREADS, 0, st>>>(in, rp, rs, cp, cs, rows, cols, mm); break;
-        case MOR_FMT_E5M2: k_mx_dual<FMT_E5M2, TILE_ROWS, DUAL_THREADS><<<(unsigned)tiles, DUAL_THREADS, 0, st>>>(in, rp, rs, cp, cs, rows, cols, mm); break;
-        case MOR_FMT_E3M2: k_mx_dual<FMT_E3M2, TILE_ROWS, DUAL_THREADS><<<(unsigned)tiles, DUAL_THREADS, 0, st>>>(in, rp, rs, cp, cs, rows, cols, mm); break;
-        default: k_mx_dual<FMT_E2M3, TILE_ROWS, DUAL_THREADS><<<(unsigned)tiles, DUAL_THREADS, 0, st>>>(in, rp, rs, cp, cs, rows, cols, mm); break;
+        case MOR_FMT_E4M3: return launch_dual<FMT_E4M3, FMT_E4M3>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+        case MOR_FMT_E5M2: return launch_dual<FMT_E5M2, FMT_E5M2>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+        case MOR_FMT_E3M2: return launch_dual<FMT_E3M2, FMT_E3M2>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+        case MOR_FMT_E2M3: return launch_dual<FMT_E2M3, FMT_E2M3>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+        default: return launch_dual<FMT_E2M1, FMT_E2M1>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
     }
-    return mor_check_launch("k_mx_dual");
+}
+
+extern "C" int mor_mx_quantize_dual_ragged(const void* input, void* row_payload, void* row_scales, void* col_payload, void* col_scales,
+                                           int64_t rows, int64_t cols, int row_fmt, int col_fmt, void* stream) {
+    if (int rc = validate_wire(input, row_payload, row_scales, rows, cols, row_fmt, 1)) return rc;
+    if (int rc = validate_wire(input, col_payload, col_scales, rows, cols, col_fmt, 1)) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (row_fmt == MOR_FMT_E4M3 && col_fmt == MOR_FMT_E4M3) return launch_dual<FMT_E4M3, FMT_E4M3>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+    if (row_fmt == MOR_FMT_E5M2 && col_fmt == MOR_FMT_E5M2) return launch_dual<FMT_E5M2, FMT_E5M2>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+    if (row_fmt == MOR_FMT_E2M1 && col_fmt == MOR_FMT_E2M1) return launch_dual<FMT_E2M1, FMT_E2M1>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+    if (row_fmt == MOR_FMT_E2M1 && col_fmt == MOR_FMT_E4M3) return launch_dual<FMT_E2M1, FMT_E4M3>(input, row_payload, row_scales, col_payload, col_scales, rows, cols, st);
+    return mor_fail(MOR_ERR_INVALID_ARGUMENT, "formats %d along rows and %d along columns: one of E4M3, E5M2, E2M1 for both, or E2M1 and E4M3", row_fmt, col_fmt);
 }
 
 extern "C" int mor_mx_dequantize(const void* payload, const void* scales, void* output, int64_t rows, int64_t cols, int fmt, void* stream) {
@@ -634,6 +759,7 @@ extern "C" int mor_mx_dequantize(const void* payload, const void* scales, void* 
     switch (fmt) {
         case MOR_FMT_E4M3: k_mx_dequantize<FMT_E4M3><<<grid, WWG, 0, st>>>(p, s, out, nchunks); break;
         case MOR_FMT_E5M2: k_mx_dequantize<FMT_E5M2><<<grid, WWG, 0, st>>>(p, s, out, nchunks); break;
+        case MOR_FMT_E2M1: k_mx_dequantize<FMT_E2M1><<<grid, WWG, 0, st>>>(p, s, out, nchunks); break;
         case MOR_FMT_E3M2: k_mx_dequantize<FMT_E3M2><<<grid, WWG, 0, st>>>(p, s, out, nchunks); break;
         default: k_mx_dequantize<FMT_E2M3><<<grid, WWG, 0, st>>>(p, s, out, nchunks); break;
     }
@@ -689,4 +815,14 @@ extern "C" int mor_selftest_hw_wire(uint64_t* mismatches, void* stream) {
     k_selftest_hw_fp8_decode<FMT_E4M3><<<(128 * 201 + WWG - 1) / WWG, WWG, 0, st>>>(reinterpret_cast<unsigned long long*>(mismatches));
     k_selftest_hw_fp8_decode<FMT_E5M2><<<(128 * 201 + WWG - 1) / WWG, WWG, 0, st>>>(reinterpret_cast<unsigned long long*>(mismatches));
     return mor_check_launch("k_selftest_hw_wire");
+}
+
+extern "C" int mor_selftest_hw_fp4(uint64_t* mismatches, void* stream) {
+    if (!mismatches) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "mismatches is NULL");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    unsigned long long* m = reinterpret_cast<unsigned long long*>(mismatches);
+    k_wire_zero_u64<<<1, 64, 0, st>>>(m, 2);
+    k_selftest_hw_fp4<<<(8192u * 253u + WWG - 1) / WWG, WWG, 0, st>>>(m);
+    k_selftest_hw_fp4_decode<<<2, WWG, 0, st>>>(m);
+    return mor_check_launch("k_selftest_hw_fp4");
 }

@@ -7,7 +7,7 @@
 namespace mor {
 
 template <int F> struct Wire {
-    static constexpr int bits = Fmt<F>::hw ? 8 : 6;
+    static constexpr int bits = Fmt<F>::hw ? 8 : (F == FMT_E2M1) ? 4 : 6;
     static constexpr int bias = (F == FMT_E4M3) ? 7 : (F == FMT_E5M2) ? 15 : (F == FMT_E3M2) ? 3 : 1;
 };
 

@@ -160,6 +160,224 @@ at::Tensor e8mx_autograd(const at::Tensor& input, int64_t dim_x, int64_t dim_y, 
         return std::vector<at::Tensor>{op.call(x, dim_x, dim_y, block_x, block_y, quantize_type, scaling_strategy)}; }))[0];
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// The MX wire format and the operators on it (mor_amd/wire.py, mor_amd/mx.py; not in the reference)
+int64_t payload_bytes(int64_t n, int64_t fmt) { return (int64_t)mor_mx_payload_bytes(1, n, (int)fmt); }
+
+// A 2-D bf16 GPU tensor, contiguous and 16-byte aligned (a view that is not is copied)
+at::Tensor wire_input(const at::Tensor& t, const char* what) {
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.is_cuda(), "mor: ", what, " must be a 2-D bfloat16 GPU tensor, got ",
+                t.scalar_type(), " ", t.sizes());
+    TORCH_CHECK(t.size(1) > 0 && t.size(1) % 32 == 0, "mor: ", what, ": MX blocks need columns that are a multiple of 32, got ", t.sizes());
+    const at::Tensor x = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15u) ? x.clone() : x;
+}
+
+std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor& input, int64_t fmt) {
+    const at::Tensor x = wire_input(input, "input");
+    TORCH_CHECK(fmt >= MOR_FMT_E4M3 && fmt <= MOR_FMT_E2M1, "mor: unknown element format ", fmt);
+    const c10::OptionalDeviceGuard guard(x.device());
+    const auto u8 = x.options().dtype(at::kByte);
+    const int64_t rows = x.size(0), cols = x.size(1);
+    at::Tensor p = at::empty({rows, payload_bytes(cols, fmt)}, u8), s = at::empty({rows, cols / 32}, u8);
+    if (rows) check(mor_mx_quantize(x.data_ptr(), p.data_ptr(), s.data_ptr(), rows, cols, (int)fmt, stream_of(x)));
+    return {p, s};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> mx_quantize_dual(const at::Tensor& input, int64_t row_fmt, int64_t col_fmt) {
+    const at::Tensor x = wire_input(input, "input");
+    const c10::OptionalDeviceGuard guard(x.device());
+    const auto u8 = x.options().dtype(at::kByte);
+    const int64_t rows = x.size(0), cols = x.size(1), blocks = cdiv(rows, 32);
+    at::Tensor rp = at::empty({rows, payload_bytes(cols, row_fmt)}, u8), rs = at::empty({rows, cols / 32}, u8);
+    at::Tensor cp = at::empty({cols, rows ? payload_bytes(blocks * 32, col_fmt) : 0}, u8), cs = at::empty({cols, blocks}, u8);
+    if (rows) check(mor_mx_quantize_dual_ragged(x.data_ptr(), rp.data_ptr(), rs.data_ptr(), cp.data_ptr(), cs.data_ptr(), rows, cols,
+                                                (int)row_fmt, (int)col_fmt, stream_of(x)));
+    return {rp, rs, cp, cs};
+}
+
+at::Tensor mx_dequantize(const at::Tensor& payload, const at::Tensor& scales, int64_t fmt) {
+    TORCH_CHECK(payload.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && payload.is_cuda() && payload.device() == scales.device() && scales.dim() == 2,
+                "mor: expected uint8 GPU tensors");
+    TORCH_CHECK(fmt >= MOR_FMT_E4M3 && fmt <= MOR_FMT_E2M1, "mor: unknown element format ", fmt);
+    const int64_t rows = scales.size(0), cols = scales.size(1) * 32;
+    TORCH_CHECK(payload.numel() == (cols ? rows * payload_bytes(cols, fmt) : 0), "mor: payload size does not match the scales");
+    const at::Tensor p = payload.contiguous(), s = scales.contiguous();
+    const c10::OptionalDeviceGuard guard(p.device());
+    at::Tensor out = at::empty({rows, cols}, p.options().dtype(at::kBFloat16));
+    if (rows) check(mor_mx_dequantize(p.data_ptr(), s.data_ptr(), out.data_ptr(), rows, cols, (int)fmt, stream_of(p)));
+    return out;
+}
+
+at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b, const at::Tensor& b_scales, int64_t a_fmt, int64_t b_fmt) {
+    auto side = [](const at::Tensor& p, const at::Tensor& s, int64_t fmt, const char* what) {
+        TORCH_CHECK(p.scalar_type() == at::kByte && s.scalar_type() == at::kByte && p.is_cuda() && p.device() == s.device() && p.dim() == 2 && s.dim() == 2,
+                    "mor: ", what, ": expected a 2-D uint8 payload and 2-D uint8 scales on one GPU");
+        TORCH_CHECK(fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E5M2 || fmt == MOR_FMT_E2M1, "mor: ", what, ": products take the formats E4M3, E5M2 and E2M1, got ", fmt);
+        TORCH_CHECK(p.size(0) == s.size(0) && p.size(1) == s.size(1) * (fmt == MOR_FMT_E2M1 ? 16 : 32), "mor: ", what, ": payload ", p.sizes(),
+                    " does not match scales ", s.sizes());
+    };
+    side(a, a_scales, a_fmt, "a");
+    side(b, b_scales, b_fmt, "b");
+    TORCH_CHECK(a.device() == b.device(), "mor: a and b must be on one device");
+    TORCH_CHECK(a_scales.size(1) == b_scales.size(1), "mor: a and b must have the same number of columns, got ", a_scales.size(1) * 32, " and ", b_scales.size(1) * 32);
+    const at::Tensor pa = a.contiguous(), sa = a_scales.contiguous(), pb = b.contiguous(), sb = b_scales.contiguous();
+    const c10::OptionalDeviceGuard guard(pa.device());
+    const int64_t m = pa.size(0), n = pb.size(0), k = sa.size(1) * 32;
+    const auto options = pa.options().dtype(at::kBFloat16);
+    if (k == 0) return at::zeros({m, n}, options);
+    at::Tensor out = at::empty({m, n}, options);
+    if (m == 0 || n == 0) return out;
+    const size_t nbytes = mor_mx_matmul_workspace_bytes(m, n, k, (int)a_fmt, (int)b_fmt);
+    at::Tensor ws;
+    if (nbytes) ws = at::empty({(int64_t)nbytes}, pa.options());
+    check(mor_mx_matmul(pa.data_ptr(), sa.data_ptr(), (int)a_fmt, pb.data_ptr(), sb.data_ptr(), (int)b_fmt, out.data_ptr(), m, n, k,
+                        nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(pa)));
+    return out;
+}
+
+// rows of contiguous elements at one stride, as they lie; anything else is copied
+at::Tensor rows_of(const at::Tensor& t, const char* what) {
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.is_cuda(), "mor: ", what, " must be a 2-D bfloat16 GPU tensor, got ",
+                t.scalar_type(), " ", t.sizes());
+    const bool as_is = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+    return as_is ? t : t.contiguous();
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+std::vector<at::Tensor> swiglu_forward(const at::Tensor& gate, const at::Tensor& up, bool keep) {
+    const at::Tensor g = rows_of(gate, "gate"), u = rows_of(up, "up");
+    TORCH_CHECK(g.sizes() == u.sizes() && g.device() == u.device(), "mor: gate and up must have the same shape and device, got ", g.sizes(), " and ", u.sizes());
+    const c10::OptionalDeviceGuard guard(g.device());
+    const int64_t rows = g.size(0), cols = g.size(1), blocks = cdiv(cols, 32);
+    const auto u8 = g.options().dtype(at::kByte);
+    at::Tensor out = at::empty({rows, cols}, g.options());
+    if (!keep) {
+        if (out.numel()) check(mor_swiglu_mx(g.data_ptr(), row_stride(g), u.data_ptr(), row_stride(u), out.data_ptr(), nullptr, nullptr, nullptr, nullptr, rows, cols, stream_of(g)));
+        return {out};
+    }
+    at::Tensor gc = at::empty({rows, blocks * 32}, u8), uc = at::empty_like(gc), gs = at::empty({rows, blocks}, u8), us = at::empty_like(gs);
+    if (out.numel()) check(mor_swiglu_mx(g.data_ptr(), row_stride(g), u.data_ptr(), row_stride(u), out.data_ptr(), gc.data_ptr(), gs.data_ptr(),
+                                         uc.data_ptr(), us.data_ptr(), rows, cols, stream_of(g)));
+    return {out, gc, gs, uc, us};
+}
+
+std::tuple<at::Tensor, at::Tensor> swiglu_backward(const at::Tensor& grad, const at::Tensor& gc, const at::Tensor& gs, const at::Tensor& uc, const at::Tensor& us) {
+    TORCH_CHECK(grad.scalar_type() == at::kBFloat16 && grad.dim() == 2 && grad.is_cuda(), "mor: grad must be a 2-D bfloat16 GPU tensor, got ", grad.scalar_type(), " ", grad.sizes());
+    const at::Tensor d = grad.contiguous();
+    const int64_t rows = d.size(0), cols = d.size(1), blocks = cdiv(cols, 32);
+    for (const at::Tensor* t : {&gc, &uc})
+        TORCH_CHECK(t->scalar_type() == at::kByte && t->device() == d.device() && t->is_contiguous() && t->sizes() == at::IntArrayRef({rows, blocks * 32}), "mor: codes do not match grad");
+    for (const at::Tensor* t : {&gs, &us})
+        TORCH_CHECK(t->scalar_type() == at::kByte && t->device() == d.device() && t->is_contiguous() && t->sizes() == at::IntArrayRef({rows, blocks}), "mor: scales do not match grad");
+    const c10::OptionalDeviceGuard guard(d.device());
+    at::Tensor dg = at::empty({rows, cols}, d.options()), du = at::empty({rows, cols}, d.options());
+    if (d.numel()) check(mor_swiglu_mx_backward(d.data_ptr(), gc.data_ptr(), gs.data_ptr(), uc.data_ptr(), us.data_ptr(), dg.data_ptr(), du.data_ptr(), rows, cols, stream_of(d)));
+    return {dg, du};
+}
+
+// the operators above through the dispatcher, so that fake tensors trace
+template <class Sig> c10::TypedOperatorHandle<Sig> handle(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>(); }
+std::tuple<at::Tensor, at::Tensor> call_quantize(const at::Tensor& x, int64_t fmt) {
+    static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t)>("mor::mx_quantize");
+    return op.call(x, fmt);
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> call_dual(const at::Tensor& x, int64_t row_fmt, int64_t col_fmt) {
+    static auto op = handle<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>(const at::Tensor&, int64_t, int64_t)>("mor::mx_quantize_dual");
+    return op.call(x, row_fmt, col_fmt);
+}
+at::Tensor call_matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, int64_t a_fmt, int64_t b_fmt) {
+    static auto op = handle<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t)>("mor::mx_matmul");
+    return op.call(a, sa, b, sb, a_fmt, b_fmt);
+}
+
+void check_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
+    TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.is_cuda() && x.dim() == 2, "mor: x must be a bfloat16 GPU tensor, got ", x.scalar_type());
+    TORCH_CHECK(w.scalar_type() == at::kBFloat16 && w.device() == x.device() && w.dim() == 2, "mor: weight must be a 2-D bfloat16 tensor on the device of x, got ",
+                w.scalar_type(), " ", w.sizes());
+    TORCH_CHECK(x.size(1) == w.size(1), "mor: x has ", x.size(1), " columns, weight has ", w.size(1));
+    TORCH_CHECK(w.size(0) > 0 && w.size(0) % 32 == 0 && w.size(1) > 0 && w.size(1) % 32 == 0, "mor: inputs and outputs must be multiples of 32, got weight ", w.sizes());
+    TORCH_CHECK(fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E2M1, "mor: fmt must be E4M3 or E2M1, got ", fmt);
+    TORCH_CHECK(grad_fmt == MOR_FMT_E4M3 || grad_fmt == MOR_FMT_E5M2, "mor: grad_fmt must be E4M3 or E5M2, got ", grad_fmt);
+}
+
+at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
+    check_linear(x, w, fmt, grad_fmt);
+    auto [xp, xs] = call_quantize(x, fmt);
+    auto [wp, ws] = call_quantize(w, fmt);
+    return call_matmul(xp, xs, wp, ws, fmt, fmt);
+}
+
+// y = Q(x) Q(w)^T.  What is kept for the backward pass: x^T in E4M3 blocks along the tokens (1.03 bytes per element) if
+// the weight wants a gradient, w^T in blocks along the outputs if x does.  The quantisers are passed straight through.
+struct MxLinear : public torch::autograd::Function<MxLinear> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt,
+                              bool need_x, bool need_w) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        at::Tensor xp, xs, xtp, xts, wp, ws, wtp, wts;
+        if (need_w) std::tie(xp, xs, xtp, xts) = call_dual(x, fmt, MOR_FMT_E4M3);
+        else std::tie(xp, xs) = call_quantize(x, fmt);
+        if (need_x) std::tie(wp, ws, wtp, wts) = call_dual(w, fmt, fmt);
+        else std::tie(wp, ws) = call_quantize(w, fmt);
+        ctx->save_for_backward({xtp, xts, wtp, wts});
+        ctx->saved_data["fmt"] = fmt;
+        ctx->saved_data["grad_fmt"] = grad_fmt;
+        return call_matmul(xp, xs, wp, ws, fmt, fmt);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "mor: mx.linear has no second derivative");
+        const auto saved = ctx->get_saved_variables();
+        const int64_t fmt = ctx->saved_data["fmt"].toInt(), grad_fmt = ctx->saved_data["grad_fmt"].toInt();
+        at::Tensor dx, dw;
+        if (grads[0].defined()) {
+            auto [gp, gs, gtp, gts] = call_dual(grads[0], grad_fmt, grad_fmt);
+            if (saved[2].defined()) dx = call_matmul(gp, gs, saved[2], saved[3], grad_fmt, fmt);
+            if (saved[0].defined()) dw = call_matmul(gtp, gts, saved[0], saved[1], grad_fmt, MOR_FMT_E4M3);
+        }
+        return {dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor mx_linear_autograd(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
+    check_linear(x, w, fmt, grad_fmt);
+    const bool on = at::GradMode::is_enabled(), need_x = on && x.requires_grad(), need_w = on && w.requires_grad();
+    if (!need_x && !need_w) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        static auto op = handle<at::Tensor(const at::Tensor&, const at::Tensor&, int64_t, int64_t)>("mor::mx_linear");
+        return op.call(x, w, fmt, grad_fmt);
+    }
+    return MxLinear::apply(x, w, fmt, grad_fmt, need_x, need_w);
+}
+
+std::vector<at::Tensor> call_swiglu(const at::Tensor& gate, const at::Tensor& up, bool keep) {
+    static auto op = handle<std::vector<at::Tensor>(const at::Tensor&, const at::Tensor&, bool)>("mor::swiglu_mx_forward");
+    return op.call(gate, up, keep);
+}
+struct SwigluMx : public torch::autograd::Function<SwigluMx> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& gate, const at::Tensor& up) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const auto r = call_swiglu(gate, up, true);
+        ctx->save_for_backward({r[1], r[2], r[3], r[4]});
+        return r[0];
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "mor: mx.swiglu has no second derivative");
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+        static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&)>("mor::swiglu_mx_backward");
+        const auto s = ctx->get_saved_variables();
+        auto [dg, du] = op.call(grads[0], s[0], s[1], s[2], s[3]);
+        return {dg, du};
+    }
+};
+at::Tensor swiglu(const at::Tensor& gate, const at::Tensor& up) { return call_swiglu(gate, up, false)[0]; }
+at::Tensor swiglu_autograd(const at::Tensor& gate, const at::Tensor& up) {
+    if (!at::GradMode::is_enabled() || !(gate.requires_grad() || up.requires_grad())) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return call_swiglu(gate, up, false)[0];
+    }
+    return SwigluMx::apply(gate, up);
+}
+
 }  // namespace
 
 // mor.ops.set_flavour: MOR_FLAG_* bits for every later call of the calling thread
@@ -186,6 +404,14 @@ TORCH_LIBRARY_IMPL(mor, CUDA, m) {
         return e8mx_impl(i, x, y, bx, by, q, s, nullptr); });
     m.impl("fake_quantize_e8mx_inplace", [](const at::Tensor& i, int64_t x, int64_t y, int64_t bx, int64_t by, int64_t q, int64_t s, at::Tensor result) {
         e8mx_impl(i, x, y, bx, by, q, s, &result); });
+    m.impl("mx_quantize", &mx_quantize);
+    m.impl("mx_quantize_dual", &mx_quantize_dual);
+    m.impl("mx_dequantize", &mx_dequantize);
+    m.impl("mx_matmul", &mx_matmul);
+    m.impl("mx_linear", &mx_linear);
+    m.impl("swiglu_mx", &swiglu);
+    m.impl("swiglu_mx_forward", &swiglu_forward);
+    m.impl("swiglu_mx_backward", &swiglu_backward);
 }
 
 // autograd for the four differentiable forward ops; the in-place / no_alloc / test ops keep their Python registration
@@ -194,4 +420,6 @@ TORCH_LIBRARY_IMPL(mor, Autograd, m) {
     m.impl("fake_quantize_block_scaling", &scaling_autograd<false>);
     m.impl("fake_quantize_channel_scaling", &scaling_autograd<true>);
     m.impl("fake_quantize_e8mx", &e8mx_autograd);
+    m.impl("mx_linear", &mx_linear_autograd);
+    m.impl("swiglu_mx", &swiglu_autograd);
 }

@@ -68,6 +68,16 @@ _lib.define("fake_quantize_e8mx_inplace(Tensor input, int dim_x, int dim_y, int 
 _lib.define("fake_quantize_channel_scaling(Tensor input, int dim_x, int dim_y, int block_x, int block_y, float e4m3_threshold, int ss_mode) -> Tensor[]")
 _lib.define("fake_quantize_channel_scaling_inplace(Tensor input, int dim_x, int dim_y, int block_x, int block_y, float e4m3_threshold, int ss_mode) -> Tensor[]")
 
+# The MX wire format and the operators on it (mor_amd/wire.py, mor_amd/mx.py; not in the reference)
+_lib.define("mx_quantize(Tensor input, int fmt) -> (Tensor, Tensor)")
+_lib.define("mx_quantize_dual(Tensor input, int row_fmt, int col_fmt) -> (Tensor, Tensor, Tensor, Tensor)")
+_lib.define("mx_dequantize(Tensor payload, Tensor scales, int fmt) -> Tensor")
+_lib.define("mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int a_fmt, int b_fmt) -> Tensor")
+_lib.define("mx_linear(Tensor x, Tensor weight, int fmt, int grad_fmt) -> Tensor")
+_lib.define("swiglu_mx(Tensor gate, Tensor up) -> Tensor")
+_lib.define("swiglu_mx_forward(Tensor gate, Tensor up, bool keep) -> Tensor[]")
+_lib.define("swiglu_mx_backward(Tensor grad, Tensor gate_codes, Tensor gate_scales, Tensor up_codes, Tensor up_scales) -> (Tensor, Tensor)")
+
 
 # ----------------------------------------------------------------------------------------------------------------------
 # Implementations for the CUDA dispatch key (which HIP tensors use under ROCm), FQ:2663-2678: the C++ registrations of
@@ -123,6 +133,28 @@ torch.library.register_fake("mor::fake_quantize_e8mx")(lambda i, x, y, bx, by, q
 for _name in ("quant_dequant_e4m3", "quant_dequant_e5m2", "quant_dequant_e3m2", "quant_dequant_e2m3",
               "e4m3_with_e8_scale_rne", "e4m3_with_e8_scale_rz"):
     torch.library.register_fake(f"mor::{_name}")(lambda i, x, y, bx, by: _fake_like(i))
+
+
+def _fake_codes(t, rows, cols, fmt):
+    bits = 4 if fmt == _cabi.FMT_E2M1 else 8 if fmt in (_cabi.FMT_E4M3, _cabi.FMT_E5M2) else 6
+    return [t.new_empty((rows, cols // 8 * bits), dtype=torch.uint8), t.new_empty((rows, cols // 32), dtype=torch.uint8)]
+
+
+def _fake_swiglu(gate, up, keep):
+    rows, wide = gate.shape[0], _cdiv(gate.shape[1], 32) * 32
+    kept = _fake_codes(gate, rows, wide, _cabi.FMT_E4M3) + _fake_codes(gate, rows, wide, _cabi.FMT_E4M3) if keep else []
+    return [_fake_like(gate)] + kept
+
+
+torch.library.register_fake("mor::mx_quantize")(lambda x, fmt: tuple(_fake_codes(x, *x.shape, fmt)))
+torch.library.register_fake("mor::mx_quantize_dual")(
+    lambda x, rf, cf: tuple(_fake_codes(x, *x.shape, rf) + _fake_codes(x, x.shape[1], _cdiv(x.shape[0], 32) * 32, cf)))
+torch.library.register_fake("mor::mx_dequantize")(lambda p, s, fmt: p.new_empty((s.shape[0], s.shape[1] * 32), dtype=torch.bfloat16))
+torch.library.register_fake("mor::mx_matmul")(lambda a, sa, b, sb, fa, fb: a.new_empty((a.shape[0], b.shape[0]), dtype=torch.bfloat16))
+torch.library.register_fake("mor::mx_linear")(lambda x, w, fmt, gf: x.new_empty((x.shape[0], w.shape[0])))
+torch.library.register_fake("mor::swiglu_mx")(lambda gate, up: _fake_like(gate))
+torch.library.register_fake("mor::swiglu_mx_forward")(_fake_swiglu)
+torch.library.register_fake("mor::swiglu_mx_backward")(lambda d, gc, gs, uc, us: (_fake_like(d), _fake_like(d)))
 
 
 # ----------------------------------------------------------------------------------------------------------------------

@@ -6,7 +6,7 @@ mor/csrc/cuda/fake_quantize.cu:801-823, :251-252): blocks of 32 elements, scale 
 `dequantize_mx(*quantize_mx(x, fmt), fmt)` equals `mor.ops.fake_quantize(x, ..., 1, 32, 0.0, mode, 2)[0]` (mode 2 for
 E4M3, 3 for E5M2) wherever the latter's values are not the exponent-clamp artefacts of that kernel.
 """
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -14,12 +14,14 @@ from torch import Tensor
 from . import _cabi
 
 E4M3, E5M2, E3M2, E2M3 = _cabi.FMT_E4M3, _cabi.FMT_E5M2, _cabi.FMT_E3M2, _cabi.FMT_E2M3
+E2M1 = _cabi.FMT_E2M1          # 4-bit codes, two to a byte; the wire format only
 
 _L = _cabi.lib()
+_op = torch.ops.mor
 
 
 def payload_row_bytes(cols: int, fmt: int) -> int:
-    return cols if fmt in (E4M3, E5M2) else cols // 4 * 3
+    return cols if fmt in (E4M3, E5M2) else cols // 2 if fmt == E2M1 else cols // 4 * 3
 
 
 def _check(x: Tensor, row_multiple: int) -> Tuple[int, int]:
@@ -73,6 +75,14 @@ def dequantize_mx(payload: Tensor, scales: Tensor, fmt: int = E4M3) -> Tensor:
         out = torch.empty((rows, cols), dtype=torch.bfloat16, device=payload.device)
         _cabi.check(_L.mor_mx_dequantize(payload.data_ptr(), scales.data_ptr(), out.data_ptr(), rows, cols, fmt, _stream(payload)))
     return out
+
+
+def matmul_mx(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, a_fmt: int = E4M3, b_fmt: Optional[int] = None) -> Tensor:
+    """a b^T of two tensors in the wire format -> bfloat16 [m, n]: payloads [m, k * bits / 8] and [n, k * bits / 8] and
+    scales [m, k / 32] and [n, k / 32] as quantize_mx gives them.  Formats E4M3, E5M2 and E2M1 in any pair (b_fmt: that
+    of a when not given).  The scaled matrix instructions read codes and scale bytes as they are, sum in fp32, and the
+    sum is rounded once; the same operands give the same bits.  A NaN in a row of a or b makes that row or column NaN."""
+    return _op.mx_matmul(a, a_scales, b, b_scales, a_fmt, a_fmt if b_fmt is None else b_fmt)
 
 
 def fake_quantize_mx_dual(x: Tensor, mode: int = 2, sf_type: int = 2) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
