@@ -9,15 +9,16 @@ the benchmark never run a library that lags behind the sources.
 import glob
 import hashlib
 import os
+import re
 import subprocess
 from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, "csrc")
 _ROOT = os.path.dirname(_HERE)
-SOURCES = [os.path.join(_CSRC, n) for n in ("mor_kernels.hip", "mor_wgblock.hip", "mor_subblock.hip", "mor_scaling.hip", "mor_wire.hip", "mor_batch.hip", "mor_dual.hip", "mor_morwire.hip", "mor_mfma_check.hip", "mor_mxmatmul.hip", "mor_swiglu.hip")]
+SOURCES = [os.path.join(_CSRC, n) for n in ("mor_kernels.hip", "mor_wgblock.hip", "mor_subblock.hip", "mor_scaling.hip", "mor_wire.hip", "mor_batch.hip", "mor_dual.hip", "mor_morwire.hip", "mor_mfma_check.hip", "mor_mxmatmul.hip", "mor_mxmatmul_e4m3.hip", "mor_mxmatmul_e5m2.hip", "mor_mxmatmul_e2m1.hip", "mor_swiglu.hip")]
 SOURCES = [s for s in SOURCES if os.path.exists(s)]
-HEADERS = [os.path.join(_CSRC, n) for n in ("mor_device.h", "mor_common.h", "mor_quant.h", "mor_wgblock.h", "mor_wirefmt.h", "mor_host.h")] + [os.path.join(_ROOT, "include", "mor_hip.h")]
+HEADERS = [os.path.join(_CSRC, n) for n in ("mor_device.h", "mor_common.h", "mor_quant.h", "mor_wgblock.h", "mor_wirefmt.h", "mor_mxmatmul.h", "mor_host.h")] + [os.path.join(_ROOT, "include", "mor_hip.h")]
 VERSION_SRC = os.path.join(_CSRC, "mor_version.cpp")
 OUT = os.path.join(_HERE, "lib", "libmor_hip.so")
 HASH_FILE = os.path.join(_HERE, "lib", "libmor_hip.srchash")           # the source hash libmor_hip.so was built from
@@ -66,8 +67,20 @@ def _read(path):
         return ""
 
 
+def _with_includes(path, seen=None):
+    """The file and the project headers it includes, directly or through another (#include "...")."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path not in seen:
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M):
+                _with_includes(os.path.join(os.path.dirname(path), name), seen)
+    return sorted(seen)
+
+
 def _obj_of(src):
-    return os.path.join(OBJ_DIR, f"{os.path.basename(src)}.{_digest([src] + HEADERS, ' '.join(HIPCC_FLAGS))}.o")
+    return os.path.join(OBJ_DIR, f"{os.path.basename(src)}.{_digest(_with_includes(src), ' '.join(HIPCC_FLAGS))}.o")
 
 
 def build_hip(verbose=False, force=True):
