@@ -191,8 +191,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> mx_quantize_dual(cons
     const int64_t rows = x.size(0), cols = x.size(1), blocks = cdiv(rows, 32);
     at::Tensor rp = at::empty({rows, payload_bytes(cols, row_fmt)}, u8), rs = at::empty({rows, cols / 32}, u8);
     at::Tensor cp = at::empty({cols, rows ? payload_bytes(blocks * 32, col_fmt) : 0}, u8), cs = at::empty({cols, blocks}, u8);
-    if (rows) check(mor_mx_quantize_dual_ragged(x.data_ptr(), rp.data_ptr(), rs.data_ptr(), cp.data_ptr(), cs.data_ptr(), rows, cols,
-                                                (int)row_fmt, (int)col_fmt, stream_of(x)));
+    if (rows && row_fmt == col_fmt && rows % 32 == 0)
+        check(mor_mx_quantize_dual(x.data_ptr(), rp.data_ptr(), rs.data_ptr(), cp.data_ptr(), cs.data_ptr(), rows, cols, (int)row_fmt, stream_of(x)));
+    else if (rows) check(mor_mx_quantize_dual_ragged(x.data_ptr(), rp.data_ptr(), rs.data_ptr(), cp.data_ptr(), cs.data_ptr(), rows, cols,
+                                                     (int)row_fmt, (int)col_fmt, stream_of(x)));
     return {rp, rs, cp, cs};
 }
 
@@ -245,135 +247,202 @@ at::Tensor rows_of(const at::Tensor& t, const char* what) {
 }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
-std::vector<at::Tensor> swiglu_forward(const at::Tensor& gate, const at::Tensor& up, bool keep) {
+// The 8-bit copies of gate and up in one buffer: codes of gate, of up, scale bytes of gate, of up
+struct SwigluKept {
+    int64_t codes, scales, bytes;
+    SwigluKept(int64_t rows, int64_t cols) : codes((rows * cdiv(cols, 32) * 32 + 255) / 256 * 256), scales(rows * cdiv(cols, 32)), bytes(2 * (codes + scales)) {}
+};
+
+std::tuple<at::Tensor, at::Tensor> swiglu_forward(const at::Tensor& gate, const at::Tensor& up, bool keep) {
     const at::Tensor g = rows_of(gate, "gate"), u = rows_of(up, "up");
     TORCH_CHECK(g.sizes() == u.sizes() && g.device() == u.device(), "mor: gate and up must have the same shape and device, got ", g.sizes(), " and ", u.sizes());
     const c10::OptionalDeviceGuard guard(g.device());
-    const int64_t rows = g.size(0), cols = g.size(1), blocks = cdiv(cols, 32);
-    const auto u8 = g.options().dtype(at::kByte);
+    const int64_t rows = g.size(0), cols = g.size(1);
     at::Tensor out = at::empty({rows, cols}, g.options());
-    if (!keep) {
-        if (out.numel()) check(mor_swiglu_mx(g.data_ptr(), row_stride(g), u.data_ptr(), row_stride(u), out.data_ptr(), nullptr, nullptr, nullptr, nullptr, rows, cols, stream_of(g)));
-        return {out};
-    }
-    at::Tensor gc = at::empty({rows, blocks * 32}, u8), uc = at::empty_like(gc), gs = at::empty({rows, blocks}, u8), us = at::empty_like(gs);
-    if (out.numel()) check(mor_swiglu_mx(g.data_ptr(), row_stride(g), u.data_ptr(), row_stride(u), out.data_ptr(), gc.data_ptr(), gs.data_ptr(),
-                                         uc.data_ptr(), us.data_ptr(), rows, cols, stream_of(g)));
-    return {out, gc, gs, uc, us};
+    const SwigluKept k(rows, cols);
+    at::Tensor kept = at::empty({keep ? k.bytes : 0}, g.options().dtype(at::kByte));
+    uint8_t* b = keep ? kept.data_ptr<uint8_t>() : nullptr;
+    if (out.numel()) check(mor_swiglu_mx(g.data_ptr(), row_stride(g), u.data_ptr(), row_stride(u), out.data_ptr(), b, b ? b + 2 * k.codes : nullptr,
+                                         b ? b + k.codes : nullptr, b ? b + 2 * k.codes + k.scales : nullptr, rows, cols, stream_of(g)));
+    return {out, kept};
 }
 
-std::tuple<at::Tensor, at::Tensor> swiglu_backward(const at::Tensor& grad, const at::Tensor& gc, const at::Tensor& gs, const at::Tensor& uc, const at::Tensor& us) {
+std::tuple<at::Tensor, at::Tensor> swiglu_backward(const at::Tensor& grad, const at::Tensor& kept) {
     TORCH_CHECK(grad.scalar_type() == at::kBFloat16 && grad.dim() == 2 && grad.is_cuda(), "mor: grad must be a 2-D bfloat16 GPU tensor, got ", grad.scalar_type(), " ", grad.sizes());
     const at::Tensor d = grad.contiguous();
-    const int64_t rows = d.size(0), cols = d.size(1), blocks = cdiv(cols, 32);
-    for (const at::Tensor* t : {&gc, &uc})
-        TORCH_CHECK(t->scalar_type() == at::kByte && t->device() == d.device() && t->is_contiguous() && t->sizes() == at::IntArrayRef({rows, blocks * 32}), "mor: codes do not match grad");
-    for (const at::Tensor* t : {&gs, &us})
-        TORCH_CHECK(t->scalar_type() == at::kByte && t->device() == d.device() && t->is_contiguous() && t->sizes() == at::IntArrayRef({rows, blocks}), "mor: scales do not match grad");
+    const int64_t rows = d.size(0), cols = d.size(1);
+    const SwigluKept k(rows, cols);
+    TORCH_CHECK(kept.scalar_type() == at::kByte && kept.device() == d.device() && kept.is_contiguous() && kept.numel() == k.bytes, "mor: kept does not match grad");
     const c10::OptionalDeviceGuard guard(d.device());
     at::Tensor dg = at::empty({rows, cols}, d.options()), du = at::empty({rows, cols}, d.options());
-    if (d.numel()) check(mor_swiglu_mx_backward(d.data_ptr(), gc.data_ptr(), gs.data_ptr(), uc.data_ptr(), us.data_ptr(), dg.data_ptr(), du.data_ptr(), rows, cols, stream_of(d)));
+    const uint8_t* b = kept.data_ptr<uint8_t>();
+    if (d.numel()) check(mor_swiglu_mx_backward(d.data_ptr(), b, b + 2 * k.codes, b + k.codes, b + 2 * k.codes + k.scales, dg.data_ptr(), du.data_ptr(), rows, cols, stream_of(d)));
     return {dg, du};
 }
 
-// the operators above through the dispatcher, so that fake tensors trace
-template <class Sig> c10::TypedOperatorHandle<Sig> handle(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>(); }
-std::tuple<at::Tensor, at::Tensor> call_quantize(const at::Tensor& x, int64_t fmt) {
-    static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t)>("mor::mx_quantize");
-    return op.call(x, fmt);
+// The linear layer.  Its codes lie in one buffer per lifetime (an allocation costs as much host time as a launch): those
+// of the forward product, those that the backward pass needs, those of dy.
+struct Parts {
+    int64_t bytes = 0;
+    int64_t add(int64_t n) { const int64_t at = bytes; bytes += (n + 255) / 256 * 256; return at; }
+};
+struct Codes { uint8_t *payload, *scales; };
+struct CodesAt {
+    int64_t payload, scales;
+    static CodesAt in(Parts& p, int64_t rows, int64_t cols, int64_t fmt) {
+        const int64_t a = p.add(rows && cols ? rows * payload_bytes(cols, fmt) : 0);
+        return {a, p.add(rows * (cols / 32))};
+    }
+    Codes of(const at::Tensor& buffer) const { uint8_t* b = buffer.data_ptr<uint8_t>(); return {b + payload, b + scales}; }
+};
+struct Kept {          // x^T [inputs, tokens filled up to blocks] in E4M3 and weight^T [inputs, outputs] in fmt
+    Parts parts;
+    CodesAt xt{}, wt{};
+    Kept(int64_t tokens, int64_t inputs, int64_t outputs, int64_t fmt, bool keep_x, bool keep_w) {
+        if (keep_x) xt = CodesAt::in(parts, inputs, cdiv(tokens, 32) * 32, MOR_FMT_E4M3);
+        if (keep_w) wt = CodesAt::in(parts, inputs, outputs, fmt);
+    }
+};
+
+void quantize_into(const at::Tensor& x, int64_t fmt, Codes rows) {
+    check(mor_mx_quantize(x.data_ptr(), rows.payload, rows.scales, x.size(0), x.size(1), (int)fmt, stream_of(x)));
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> call_dual(const at::Tensor& x, int64_t row_fmt, int64_t col_fmt) {
-    static auto op = handle<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>(const at::Tensor&, int64_t, int64_t)>("mor::mx_quantize_dual");
-    return op.call(x, row_fmt, col_fmt);
+void quantize_into(const at::Tensor& x, int64_t row_fmt, Codes rows, int64_t col_fmt, Codes cols) {
+    check(mor_mx_quantize_dual_ragged(x.data_ptr(), rows.payload, rows.scales, cols.payload, cols.scales, x.size(0), x.size(1), (int)row_fmt, (int)col_fmt, stream_of(x)));
 }
-at::Tensor call_matmul(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, int64_t a_fmt, int64_t b_fmt) {
-    static auto op = handle<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t)>("mor::mx_matmul");
-    return op.call(a, sa, b, sb, a_fmt, b_fmt);
+at::Tensor product(Codes a, int64_t a_fmt, Codes b, int64_t b_fmt, int64_t m, int64_t n, int64_t k, const at::TensorOptions& options, void* stream) {
+    at::Tensor out = at::empty({m, n}, options.dtype(at::kBFloat16)), ws;
+    const size_t nbytes = mor_mx_matmul_workspace_bytes(m, n, k, (int)a_fmt, (int)b_fmt);
+    if (nbytes) ws = at::empty({(int64_t)nbytes}, options.dtype(at::kByte));
+    check(mor_mx_matmul(a.payload, a.scales, (int)a_fmt, b.payload, b.scales, (int)b_fmt, out.data_ptr(), m, n, k, nbytes ? ws.data_ptr() : nullptr, nbytes, stream));
+    return out;
 }
 
-void check_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
+void check_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt) {
     TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.is_cuda() && x.dim() == 2, "mor: x must be a bfloat16 GPU tensor, got ", x.scalar_type());
     TORCH_CHECK(w.scalar_type() == at::kBFloat16 && w.device() == x.device() && w.dim() == 2, "mor: weight must be a 2-D bfloat16 tensor on the device of x, got ",
                 w.scalar_type(), " ", w.sizes());
     TORCH_CHECK(x.size(1) == w.size(1), "mor: x has ", x.size(1), " columns, weight has ", w.size(1));
     TORCH_CHECK(w.size(0) > 0 && w.size(0) % 32 == 0 && w.size(1) > 0 && w.size(1) % 32 == 0, "mor: inputs and outputs must be multiples of 32, got weight ", w.sizes());
     TORCH_CHECK(fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E2M1, "mor: fmt must be E4M3 or E2M1, got ", fmt);
-    TORCH_CHECK(grad_fmt == MOR_FMT_E4M3 || grad_fmt == MOR_FMT_E5M2, "mor: grad_fmt must be E4M3 or E5M2, got ", grad_fmt);
+}
+void check_grad_fmt(int64_t grad_fmt) { TORCH_CHECK(grad_fmt == MOR_FMT_E4M3 || grad_fmt == MOR_FMT_E5M2, "mor: grad_fmt must be E4M3 or E5M2, got ", grad_fmt); }
+
+// y = Q(x) Q(w)^T, and what the backward pass needs: x^T if the weight wants a gradient, weight^T if x does
+std::tuple<at::Tensor, at::Tensor> linear_forward(const at::Tensor& input, const at::Tensor& weight, int64_t fmt, bool keep_x, bool keep_w) {
+    check_linear(input, weight, fmt);
+    const at::Tensor x = wire_input(input, "x"), w = wire_input(weight, "weight");
+    const c10::OptionalDeviceGuard guard(x.device());
+    const int64_t tokens = x.size(0), inputs = x.size(1), outputs = w.size(0);
+    const auto u8 = x.options().dtype(at::kByte);
+    Parts scratch;
+    const CodesAt xr = CodesAt::in(scratch, tokens, inputs, fmt), wr = CodesAt::in(scratch, outputs, inputs, fmt);
+    const Kept k(tokens, inputs, outputs, fmt, keep_x, keep_w);
+    const at::Tensor rows = at::empty({scratch.bytes}, u8);
+    at::Tensor kept = at::empty({k.parts.bytes}, u8);
+    if (keep_w) quantize_into(w, fmt, wr.of(rows), fmt, k.wt.of(kept));
+    else quantize_into(w, fmt, wr.of(rows));
+    if (tokens == 0) return {at::empty({0, outputs}, x.options()), kept};
+    if (keep_x) quantize_into(x, fmt, xr.of(rows), MOR_FMT_E4M3, k.xt.of(kept));
+    else quantize_into(x, fmt, xr.of(rows));
+    return {product(xr.of(rows), fmt, wr.of(rows), fmt, tokens, outputs, inputs, u8, stream_of(x)), kept};
 }
 
+std::tuple<at::Tensor, at::Tensor> linear_backward(const at::Tensor& grad, const at::Tensor& kept, int64_t inputs, int64_t fmt, int64_t grad_fmt, bool kept_x, bool kept_w) {
+    check_grad_fmt(grad_fmt);
+    const at::Tensor d = wire_input(grad, "grad");
+    const int64_t tokens = d.size(0), outputs = d.size(1), padded = cdiv(tokens, 32) * 32;
+    const Kept k(tokens, inputs, outputs, fmt, kept_x, kept_w);
+    TORCH_CHECK(kept.scalar_type() == at::kByte && kept.device() == d.device() && kept.is_contiguous() && kept.numel() == k.parts.bytes, "mor: kept does not match grad");
+    const c10::OptionalDeviceGuard guard(d.device());
+    const auto u8 = d.options().dtype(at::kByte);
+    at::Tensor dx = at::empty({0}, d.options()), dw = dx;
+    if (tokens == 0) {
+        if (kept_w) dx = at::empty({0, inputs}, d.options());
+        if (kept_x) dw = at::zeros({outputs, inputs}, d.options());
+        return {dx, dw};
+    }
+    Parts scratch;
+    const CodesAt gr = CodesAt::in(scratch, tokens, outputs, grad_fmt), gt = kept_x ? CodesAt::in(scratch, outputs, padded, grad_fmt) : CodesAt{};
+    const at::Tensor codes = at::empty({scratch.bytes}, u8);
+    if (kept_x) quantize_into(d, grad_fmt, gr.of(codes), grad_fmt, gt.of(codes));
+    else quantize_into(d, grad_fmt, gr.of(codes));
+    if (kept_w) dx = product(gr.of(codes), grad_fmt, k.wt.of(kept), fmt, tokens, inputs, outputs, u8, stream_of(d));
+    if (kept_x) dw = product(gt.of(codes), grad_fmt, k.xt.of(kept), MOR_FMT_E4M3, outputs, inputs, padded, u8, stream_of(d));
+    return {dx, dw};
+}
+
+// the operators above through the dispatcher, so that fake tensors trace
+template <class Sig> c10::TypedOperatorHandle<Sig> handle(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>(); }
+std::tuple<at::Tensor, at::Tensor> call_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, bool keep_x, bool keep_w) {
+    static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, int64_t, bool, bool)>("mor::mx_linear_forward");
+    return op.call(x, w, fmt, keep_x, keep_w);
+}
 at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
-    check_linear(x, w, fmt, grad_fmt);
-    auto [xp, xs] = call_quantize(x, fmt);
-    auto [wp, ws] = call_quantize(w, fmt);
-    return call_matmul(xp, xs, wp, ws, fmt, fmt);
+    check_grad_fmt(grad_fmt);
+    return std::get<0>(call_linear(x, w, fmt, false, false));
 }
 
-// y = Q(x) Q(w)^T.  What is kept for the backward pass: x^T in E4M3 blocks along the tokens (1.03 bytes per element) if
-// the weight wants a gradient, w^T in blocks along the outputs if x does.  The quantisers are passed straight through.
+// The quantisers are passed straight through.
 struct MxLinear : public torch::autograd::Function<MxLinear> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt,
                               bool need_x, bool need_w) {
         at::AutoDispatchBelowADInplaceOrView below;
-        at::Tensor xp, xs, xtp, xts, wp, ws, wtp, wts;
-        if (need_w) std::tie(xp, xs, xtp, xts) = call_dual(x, fmt, MOR_FMT_E4M3);
-        else std::tie(xp, xs) = call_quantize(x, fmt);
-        if (need_x) std::tie(wp, ws, wtp, wts) = call_dual(w, fmt, fmt);
-        else std::tie(wp, ws) = call_quantize(w, fmt);
-        ctx->save_for_backward({xtp, xts, wtp, wts});
-        ctx->saved_data["fmt"] = fmt;
-        ctx->saved_data["grad_fmt"] = grad_fmt;
-        return call_matmul(xp, xs, wp, ws, fmt, fmt);
+        auto [y, kept] = call_linear(x, w, fmt, need_w, need_x);
+        ctx->save_for_backward({kept});
+        ctx->saved_data["fmts"] = fmt * 16 + grad_fmt;
+        ctx->saved_data["kept"] = (int64_t)need_w * 2 + (int64_t)need_x;
+        ctx->saved_data["inputs"] = w.size(1);
+        return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "mor: mx.linear has no second derivative");
-        const auto saved = ctx->get_saved_variables();
-        const int64_t fmt = ctx->saved_data["fmt"].toInt(), grad_fmt = ctx->saved_data["grad_fmt"].toInt();
         at::Tensor dx, dw;
         if (grads[0].defined()) {
-            auto [gp, gs, gtp, gts] = call_dual(grads[0], grad_fmt, grad_fmt);
-            if (saved[2].defined()) dx = call_matmul(gp, gs, saved[2], saved[3], grad_fmt, fmt);
-            if (saved[0].defined()) dw = call_matmul(gtp, gts, saved[0], saved[1], grad_fmt, MOR_FMT_E4M3);
+            static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, int64_t, int64_t, int64_t, bool, bool)>("mor::mx_linear_backward");
+            const int64_t fmts = ctx->saved_data["fmts"].toInt(), kept = ctx->saved_data["kept"].toInt();
+            std::tie(dx, dw) = op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["inputs"].toInt(), fmts / 16, fmts % 16, kept & 2, kept & 1);
+            if (!(kept & 1)) dx = at::Tensor();
+            if (!(kept & 2)) dw = at::Tensor();
         }
         return {dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     }
 };
 
 at::Tensor mx_linear_autograd(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
-    check_linear(x, w, fmt, grad_fmt);
+    check_grad_fmt(grad_fmt);
     const bool on = at::GradMode::is_enabled(), need_x = on && x.requires_grad(), need_w = on && w.requires_grad();
     if (!need_x && !need_w) {
         at::AutoDispatchBelowADInplaceOrView below;
-        static auto op = handle<at::Tensor(const at::Tensor&, const at::Tensor&, int64_t, int64_t)>("mor::mx_linear");
-        return op.call(x, w, fmt, grad_fmt);
+        return std::get<0>(call_linear(x, w, fmt, false, false));
     }
     return MxLinear::apply(x, w, fmt, grad_fmt, need_x, need_w);
 }
 
-std::vector<at::Tensor> call_swiglu(const at::Tensor& gate, const at::Tensor& up, bool keep) {
-    static auto op = handle<std::vector<at::Tensor>(const at::Tensor&, const at::Tensor&, bool)>("mor::swiglu_mx_forward");
+std::tuple<at::Tensor, at::Tensor> call_swiglu(const at::Tensor& gate, const at::Tensor& up, bool keep) {
+    static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, bool)>("mor::swiglu_mx_forward");
     return op.call(gate, up, keep);
 }
 struct SwigluMx : public torch::autograd::Function<SwigluMx> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& gate, const at::Tensor& up) {
         at::AutoDispatchBelowADInplaceOrView below;
-        const auto r = call_swiglu(gate, up, true);
-        ctx->save_for_backward({r[1], r[2], r[3], r[4]});
-        return r[0];
+        auto [h, kept] = call_swiglu(gate, up, true);
+        ctx->save_for_backward({kept});
+        return h;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "mor: mx.swiglu has no second derivative");
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
-        static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&)>("mor::swiglu_mx_backward");
-        const auto s = ctx->get_saved_variables();
-        auto [dg, du] = op.call(grads[0], s[0], s[1], s[2], s[3]);
+        static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&)>("mor::swiglu_mx_backward");
+        auto [dg, du] = op.call(grads[0], ctx->get_saved_variables()[0]);
         return {dg, du};
     }
 };
-at::Tensor swiglu(const at::Tensor& gate, const at::Tensor& up) { return call_swiglu(gate, up, false)[0]; }
+at::Tensor swiglu(const at::Tensor& gate, const at::Tensor& up) { return std::get<0>(call_swiglu(gate, up, false)); }
 at::Tensor swiglu_autograd(const at::Tensor& gate, const at::Tensor& up) {
     if (!at::GradMode::is_enabled() || !(gate.requires_grad() || up.requires_grad())) {
         at::AutoDispatchBelowADInplaceOrView below;
-        return call_swiglu(gate, up, false)[0];
+        return std::get<0>(call_swiglu(gate, up, false));
     }
     return SwigluMx::apply(gate, up);
 }
@@ -409,6 +478,8 @@ TORCH_LIBRARY_IMPL(mor, CUDA, m) {
     m.impl("mx_dequantize", &mx_dequantize);
     m.impl("mx_matmul", &mx_matmul);
     m.impl("mx_linear", &mx_linear);
+    m.impl("mx_linear_forward", &linear_forward);
+    m.impl("mx_linear_backward", &linear_backward);
     m.impl("swiglu_mx", &swiglu);
     m.impl("swiglu_mx_forward", &swiglu_forward);
     m.impl("swiglu_mx_backward", &swiglu_backward);

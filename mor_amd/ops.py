@@ -75,8 +75,11 @@ _lib.define("mx_dequantize(Tensor payload, Tensor scales, int fmt) -> Tensor")
 _lib.define("mx_matmul(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int a_fmt, int b_fmt) -> Tensor")
 _lib.define("mx_linear(Tensor x, Tensor weight, int fmt, int grad_fmt) -> Tensor")
 _lib.define("swiglu_mx(Tensor gate, Tensor up) -> Tensor")
-_lib.define("swiglu_mx_forward(Tensor gate, Tensor up, bool keep) -> Tensor[]")
-_lib.define("swiglu_mx_backward(Tensor grad, Tensor gate_codes, Tensor gate_scales, Tensor up_codes, Tensor up_scales) -> (Tensor, Tensor)")
+# the halves of the two above: what `keep` keeps for the backward pass is one buffer of codes and scale bytes
+_lib.define("mx_linear_forward(Tensor x, Tensor weight, int fmt, bool keep_x, bool keep_weight) -> (Tensor, Tensor)")
+_lib.define("mx_linear_backward(Tensor grad, Tensor kept, int inputs, int fmt, int grad_fmt, bool kept_x, bool kept_weight) -> (Tensor, Tensor)")
+_lib.define("swiglu_mx_forward(Tensor gate, Tensor up, bool keep) -> (Tensor, Tensor)")
+_lib.define("swiglu_mx_backward(Tensor grad, Tensor kept) -> (Tensor, Tensor)")
 
 
 # ----------------------------------------------------------------------------------------------------------------------
@@ -135,15 +138,34 @@ for _name in ("quant_dequant_e4m3", "quant_dequant_e5m2", "quant_dequant_e3m2", 
     torch.library.register_fake(f"mor::{_name}")(lambda i, x, y, bx, by: _fake_like(i))
 
 
+def _code_bits(fmt):
+    return 4 if fmt == _cabi.FMT_E2M1 else 8 if fmt in (_cabi.FMT_E4M3, _cabi.FMT_E5M2) else 6
+
+
 def _fake_codes(t, rows, cols, fmt):
-    bits = 4 if fmt == _cabi.FMT_E2M1 else 8 if fmt in (_cabi.FMT_E4M3, _cabi.FMT_E5M2) else 6
-    return [t.new_empty((rows, cols // 8 * bits), dtype=torch.uint8), t.new_empty((rows, cols // 32), dtype=torch.uint8)]
+    return [t.new_empty((rows, cols // 8 * _code_bits(fmt)), dtype=torch.uint8), t.new_empty((rows, cols // 32), dtype=torch.uint8)]
+
+
+def _up(n):
+    return _cdiv(n, 256) * 256
+
+
+# the sizes of the kept buffers: Kept and SwigluKept of csrc/torch_binding.cpp
+def _fake_linear(x, w, fmt, keep_x, keep_weight):
+    (tokens, inputs), outputs = x.shape, w.shape[0]
+    padded = _cdiv(tokens, 32) * 32
+    n = _up(inputs * padded) + _up(inputs * padded // 32) if keep_x else 0
+    n += _up(inputs * outputs // 8 * _code_bits(fmt)) + _up(inputs * outputs // 32) if keep_weight else 0
+    return x.new_empty((tokens, outputs)), x.new_empty((n,), dtype=torch.uint8)
+
+
+def _fake_linear_backward(d, kept, inputs, fmt, grad_fmt, kept_x, kept_weight):
+    return d.new_empty((d.shape[0], inputs) if kept_weight else (0,)), d.new_empty((d.shape[1], inputs) if kept_x else (0,))
 
 
 def _fake_swiglu(gate, up, keep):
-    rows, wide = gate.shape[0], _cdiv(gate.shape[1], 32) * 32
-    kept = _fake_codes(gate, rows, wide, _cabi.FMT_E4M3) + _fake_codes(gate, rows, wide, _cabi.FMT_E4M3) if keep else []
-    return [_fake_like(gate)] + kept
+    blocks = gate.shape[0] * _cdiv(gate.shape[1], 32)
+    return _fake_like(gate), gate.new_empty((2 * (_up(blocks * 32) + blocks) if keep else 0,), dtype=torch.uint8)
 
 
 torch.library.register_fake("mor::mx_quantize")(lambda x, fmt: tuple(_fake_codes(x, *x.shape, fmt)))
@@ -154,7 +176,9 @@ torch.library.register_fake("mor::mx_matmul")(lambda a, sa, b, sb, fa, fb: a.new
 torch.library.register_fake("mor::mx_linear")(lambda x, w, fmt, gf: x.new_empty((x.shape[0], w.shape[0])))
 torch.library.register_fake("mor::swiglu_mx")(lambda gate, up: _fake_like(gate))
 torch.library.register_fake("mor::swiglu_mx_forward")(_fake_swiglu)
-torch.library.register_fake("mor::swiglu_mx_backward")(lambda d, gc, gs, uc, us: (_fake_like(d), _fake_like(d)))
+torch.library.register_fake("mor::mx_linear_forward")(_fake_linear)
+torch.library.register_fake("mor::mx_linear_backward")(_fake_linear_backward)
+torch.library.register_fake("mor::swiglu_mx_backward")(lambda d, kept: (_fake_like(d), _fake_like(d)))
 
 
 # ----------------------------------------------------------------------------------------------------------------------

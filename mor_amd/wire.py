@@ -38,43 +38,22 @@ def _stream(x: Tensor) -> int:
 
 
 def quantize_mx(x: Tensor, fmt: int = E4M3) -> Tuple[Tensor, Tensor]:
-    """-> (payload uint8 [rows, cols * bits / 8], scales uint8 [rows, cols / 32]); blocks of 32 along rows."""
-    rows, cols = _check(x, 1)
-    x = x.contiguous()
-    with torch.cuda.device(x.device):
-        payload = torch.empty((rows, payload_row_bytes(cols, fmt)), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x.device)
-        _cabi.check(_L.mor_mx_quantize(x.data_ptr(), payload.data_ptr(), scales.data_ptr(), rows, cols, fmt, _stream(x)))
-    return payload, scales
+    """-> (payload uint8 [rows, cols * bits / 8], scales uint8 [rows, cols / 32]); blocks of 32 along rows.  E2M1 has two
+    codes to a byte, the first in the low half; a block with an infinity or a NaN has scale byte 255 there and decodes to
+    NaNs."""
+    return _op.mx_quantize(x, fmt)
 
 
 def quantize_mx_dual(x: Tensor, fmt: int = E4M3) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     """One read of x, both orientations: (payload, scales) of x as quantize_mx gives them and (payload, scales) of
     x.t() -- the operands of the dgrad and wgrad GEMMs of a linear layer."""
-    rows, cols = _check(x, 32)
-    x = x.contiguous()
-    with torch.cuda.device(x.device):
-        rp = torch.empty((rows, payload_row_bytes(cols, fmt)), dtype=torch.uint8, device=x.device)
-        rs = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x.device)
-        cp = torch.empty((cols, payload_row_bytes(rows, fmt)), dtype=torch.uint8, device=x.device)
-        cs = torch.empty((cols, rows // 32), dtype=torch.uint8, device=x.device)
-        _cabi.check(_L.mor_mx_quantize_dual(x.data_ptr(), rp.data_ptr(), rs.data_ptr(), cp.data_ptr(), cs.data_ptr(),
-                                            rows, cols, fmt, _stream(x)))
-    return rp, rs, cp, cs
+    _check(x, 32)
+    return _op.mx_quantize_dual(x, fmt, fmt)
 
 
 def dequantize_mx(payload: Tensor, scales: Tensor, fmt: int = E4M3) -> Tensor:
     """payload + scales -> bf16 [rows, 32 * scales.shape[1]]"""
-    if payload.dtype != torch.uint8 or scales.dtype != torch.uint8 or not payload.is_cuda or scales.dim() != 2:
-        raise RuntimeError("mor: expected uint8 GPU tensors")
-    rows, cols = scales.shape[0], scales.shape[1] * 32
-    if payload.numel() != rows * payload_row_bytes(cols, fmt):
-        raise RuntimeError("mor: payload size does not match the scales")
-    payload, scales = payload.contiguous(), scales.contiguous()
-    with torch.cuda.device(payload.device):
-        out = torch.empty((rows, cols), dtype=torch.bfloat16, device=payload.device)
-        _cabi.check(_L.mor_mx_dequantize(payload.data_ptr(), scales.data_ptr(), out.data_ptr(), rows, cols, fmt, _stream(payload)))
-    return out
+    return _op.mx_dequantize(payload, scales, fmt)
 
 
 def matmul_mx(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, a_fmt: int = E4M3, b_fmt: Optional[int] = None) -> Tensor:
