@@ -49,7 +49,8 @@ struct MxOperand {
 struct MxArgs {
     MxOperand a, b;
     const uint8_t *scales_a, *scales_b;      // k_mx_tile with T = 256: as k_mx_scales leaves them
-    uint16_t* out;                 // bf16 [a.rows, b.rows]
+    uint16_t* out;                 // bf16 [a.rows, b.rows], out_stride elements from row to row
+    int64_t out_stride;
     float* partial;                // [splits, a.rows, b.rows] when k is split, else NULL
     int k;
     int tiles_m, tiles_n;
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
             const int row = t * ROWS + lane / LANES;
             const uint4 v = *reinterpret_cast<const uint4*>(mine + row * PITCH + (lane % LANES) * 16);
             const int64_t m = m0 + wm + row;
-            if (m < p.a.rows && n < p.b.rows) store16<T == 256>(reinterpret_cast<uint4*>(p.out + m * p.b.rows + n), v);
+            if (m < p.a.rows && n < p.b.rows) store16<T == 256>(reinterpret_cast<uint4*>(p.out + m * p.out_stride + n), v);
         }
     } else {
         constexpr int LANES = WIDE / 2, ROWS = 64 / LANES;
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
             const int row = t * ROWS + lane / LANES;
             const uint32_t v = *reinterpret_cast<const uint32_t*>(mine + row * PITCH + (lane % LANES) * 4);
             const int64_t m = m0 + wm + row;
-            uint16_t* at = p.out + m * p.b.rows + n;
+            uint16_t* at = p.out + m * p.out_stride + n;
             if (m < p.a.rows && n < p.b.rows) at[0] = (uint16_t)v;
             if (m < p.a.rows && n + 1 < p.b.rows) at[1] = (uint16_t)(v >> 16);
         }
@@ -516,7 +517,7 @@ __global__ __launch_bounds__(512) void k_mx_skinny(const MxArgs p, int k_per_wav
         for (int w = 1; w < waves; ++w) v += sums[w * MT * 64 + t];
         const int64_t m = 16 * (t >> 6) + (t & 15), n = n0 + 4 * ((t >> 4) & 3);
         if (m >= p.a.rows) continue;
-        uint16_t* at = p.out + m * p.b.rows + n;
+        uint16_t* at = p.out + m * p.out_stride + n;
         const uint32_t lo = pack_bf16(v[0], v[1]), hi = pack_bf16(v[2], v[3]);
         if (p.out16) {
             if (n < p.b.rows) *reinterpret_cast<uint2*>(at) = make_uint2(lo, hi);
@@ -532,6 +533,7 @@ __global__ __launch_bounds__(512) void k_mx_skinny(const MxArgs p, int k_per_wav
 // Which kernel, and how k is divided.
 struct MxPlan {
     int tile;                      // k_mx_tile: 256 or 128; 0: k_mx_skinny
+    int64_t cut_m, cut_n;          // tile 256: the rows and columns it takes, the rest in tiles of 128
     int splits, steps_per_split;   // k_mx_tile
     int waves, k_per_wave;         // k_mx_skinny
 };

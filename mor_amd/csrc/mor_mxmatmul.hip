@@ -59,9 +59,20 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt) {
     }
     const int ks = (bits_of(a_fmt) == 4 && bits_of(b_fmt) == 4) ? 256 : 128, group = 512 / ks;
     const int64_t steps = cdiv(k, ks);
-    // 256 x 256 tiles where they occupy three quarters of the 256 CUs (4096 x 4096 x 4096 in E4M3, 256 of them: 57 us, 82 in
-    // 128 x 128 tiles; 2048 x 4096 x 4096, 128 of them: 46 us, 36 in small tiles)
-    q.tile = cdiv(m, 256) * cdiv(n, 256) >= 192 ? 256 : 128;
+    // 256 x 256 tiles where small ones would take more than one round of 512, two to a CU (2560 x 4096 x 4096 in E4M3, 160
+    // large tiles: 47 us, 55 in small ones; 2048 x 4096 x 4096, 128 of them: 46 us, 36 in small ones)
+    const int64_t large_m = cdiv(m, 256), large_n = cdiv(n, 256), large = large_m * large_n;
+    q.tile = large > 128 ? 256 : 128;
+    q.cut_m = m;
+    q.cut_n = n;
+    // A last round of large tiles on few CUs takes nearly as long as a full one: its columns or rows go to small tiles instead
+    // (4096 x 4608 x 4096 in E4M3, 288 tiles: 96 -> 82 us, 8192 x 4608, 576: 148 -> 137 us).  Of half a round that pays only
+    // after one full one (4096 x 6144, 384 tiles: 98 -> 95 us; 4096 x 14336, 896: 203 -> 209 us).
+    if (q.tile == 256 && large > 256) {
+        const int64_t full = large / 256 * 256, most = large < 512 ? 128 : 64, c_n = full / large_m, c_m = full / large_n;
+        if (large > full && large - c_n * large_m <= most) q.cut_n = std::min(n, c_n * 256);
+        else if (large > full && large - c_m * large_n <= most) q.cut_m = std::min(m, c_m * 256);
+    }
     const int64_t tiles = cdiv(m, q.tile) * cdiv(n, q.tile);
     // k is split where small tiles leave CUs idle, by the smallest of 4 us + 0.6 us a step (two workgroups share a CU
     // without slowing each other: a step waits for memory) and, when split, 3 us + 8 bytes per result and part at 4 TB/s
@@ -85,9 +96,19 @@ static size_t mx_workspace(const MxPlan& q, int64_t m, int64_t n, int64_t k) {
     return q.splits > 1 ? (size_t)q.splits * (size_t)m * (size_t)n * sizeof(float) : 0;
 }
 
+static int launch(MxArgs args, int a_fmt, int b_fmt, const MxPlan& q, hipStream_t st) {
+    args.steps_per_split = q.steps_per_split;
+    if (q.tile) {
+        args.tiles_m = (int)cdiv(args.a.rows, q.tile);
+        args.tiles_n = (int)cdiv(args.b.rows, q.tile);
+    }
+    return a_fmt == MOR_FMT_E4M3 ? launch_product_e4m3(args, b_fmt, q, st) : a_fmt == MOR_FMT_E5M2 ? launch_product_e5m2(args, b_fmt, q, st)
+                                                                                                   : launch_product_e2m1(args, b_fmt, q, st);
+}
+
 static bool product_format(int fmt) { return fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E5M2 || fmt == MOR_FMT_E2M1; }
 static bool product_shape(int64_t m, int64_t n, int64_t k) {
-    return m > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 23) && m < (1ll << 31) && n < (1ll << 31) && m <= MOR_MAX_ELEMENTS / n;
+    return m > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 23) && m < (1ll << 31) && n < (1ll << 31) && m <= MOR_MAX_ELEMENTS / n;      // (fewer than 2^25 tiles)
 }
 
 }  // namespace mor
@@ -118,30 +139,38 @@ extern "C" int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_
     args.a = {static_cast<const uint8_t*>(a_payload), static_cast<const uint8_t*>(a_scales), m};
     args.b = {static_cast<const uint8_t*>(b_payload), static_cast<const uint8_t*>(b_scales), n};
     args.out = static_cast<uint16_t*>(output);
-    if (q.tile == 256) {
-        args.scales_a = static_cast<const uint8_t*>(workspace);
-        args.scales_b = args.scales_a + (size_t)m * (size_t)cdiv(k, 512) * 16;
-    } else if (need) args.partial = static_cast<float*>(workspace);
-    args.k = (int)k;
+    args.out_stride = n;
     args.out16 = n % 8 == 0 && aligned16(output);
-    args.steps_per_split = q.steps_per_split;
-    if (q.tile) {
-        const int64_t tm = cdiv(m, q.tile), tn = cdiv(n, q.tile);
-        if (tm * tn > 0x7FFFFFFFll) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "too many tiles");
-        args.tiles_m = (int)tm;
-        args.tiles_n = (int)tn;
-    }
+    args.k = (int)k;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (q.tile == 256) {
+        const int64_t cut_m = q.cut_m, cut_n = q.cut_n;            // what the large tiles take; all of it where nothing is cut
+        MxArgs rest = args;
+        if (cut_m < m) {
+            rest.a = {args.a.payload + cut_m * (k / 8 * bits_of(a_fmt)), args.a.scales + cut_m * (k / 32), m - cut_m};
+            rest.out += cut_m * n;
+            args.a.rows = cut_m;
+        } else if (cut_n < n) {
+            rest.b = {args.b.payload + cut_n * (k / 8 * bits_of(b_fmt)), args.b.scales + cut_n * (k / 32), n - cut_n};
+            rest.out += cut_n;
+            args.b.rows = cut_n;
+        }
         const int groups = (int)cdiv(k, 512);
-        const int64_t pieces = cdiv(std::max(m, n), 16) * cdiv(groups, 16);
-        k_mx_scales<<<dim3((unsigned)std::min<int64_t>(pieces, 8192), 2), 256, 0, st>>>(
-            args.a, args.b, static_cast<uint4*>(workspace), static_cast<uint4*>(workspace) + m * groups, (int)(k / 32), groups);
+        uint4 *const scales_a = static_cast<uint4*>(workspace), *const scales_b = scales_a + cut_m * groups;
+        args.scales_a = reinterpret_cast<const uint8_t*>(scales_a);
+        args.scales_b = reinterpret_cast<const uint8_t*>(scales_b);
+        const int64_t pieces = cdiv(std::max(cut_m, cut_n), 16) * cdiv(groups, 16);
+        k_mx_scales<<<dim3((unsigned)std::min<int64_t>(pieces, 8192), 2), 256, 0, st>>>(args.a, args.b, scales_a, scales_b, (int)(k / 32), groups);
         if (int rc = mor_check_launch("k_mx_scales")) return rc;
+        if (int rc = launch(args, a_fmt, b_fmt, q, st)) return rc;
+        if (cut_m == m && cut_n == n) return MOR_OK;
+        MxPlan small = q;
+        small.tile = 128;
+        return launch(rest, a_fmt, b_fmt, small, st);
     }
-    const int rc = a_fmt == MOR_FMT_E4M3 ? launch_product_e4m3(args, b_fmt, q, st) : a_fmt == MOR_FMT_E5M2 ? launch_product_e5m2(args, b_fmt, q, st)
-                                                                                                         : launch_product_e2m1(args, b_fmt, q, st);
-    if (rc || !args.partial) return rc;
+    if (need) args.partial = static_cast<float*>(workspace);
+    if (int rc = launch(args, a_fmt, b_fmt, q, st)) return rc;
+    if (!need) return MOR_OK;
     k_mx_join<<<(unsigned)std::min<int64_t>(cdiv(m * n, 1024), 2048), 256, 0, st>>>(args.partial, args.out, m * n, q.splits);
     return mor_check_launch("k_mx_join");
 }
