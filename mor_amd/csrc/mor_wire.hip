@@ -186,6 +186,69 @@ template <int F> __device__ __forceinline__ void emit_chunk(uint8_t* payload, in
     }
 }
 
+// 8- and 4-bit formats, blocks whose scale exponent is within 2^+-100, which excludes zeros, infinities and NaNs: scale and
+// codes in few instructions.  With amax = m 2^ea and fmax = f 2^eb, e8 = eb - ea - (m > f) (make_scale_e8), so that the
+// scale byte 127 - e8 is the exponent field of amax plus the carry of (mantissa > f's), minus eb; and the byte in place of
+// an exponent is the scale that the scaled converts divide by, straight from the packed bf16 words (mor_selftest_hw_cast
+// and mor_selftest_hw_fp4 compare them with the other form).
+template <int F> struct QuickScale {
+    static constexpr uint32_t eb = F == FMT_E4M3 ? 8 : F == FMT_E5M2 ? 15 : 2, mantissa = F == FMT_E2M1 ? 0x40u : 0x60u;
+    uint32_t byte;
+    bool ok;
+    __device__ __forceinline__ explicit QuickScale(uint32_t amax_bits) {
+        byte = ((amax_bits + ((0x7Fu - mantissa) << 16)) >> 23) - eb;
+        ok = byte - 27u <= 200u;
+    }
+    __device__ __forceinline__ float value() const { return u2f(byte << 23); }
+};
+__device__ __forceinline__ uint32_t octet_amax_bits(uint4 v) {
+    uint32_t m = 0;
+    acc_amax_pk(m, v.x); acc_amax_pk(m, v.y); acc_amax_pk(m, v.z); acc_amax_pk(m, v.w);
+    return amax_bits_of(m);
+}
+// 4 codes of two packed words
+template <int F> __device__ __forceinline__ uint32_t quick_codes8(uint32_t w0, uint32_t w1, float scale) {
+    s16x2 p = {0, 0};
+    if constexpr (F == FMT_E4M3) {
+        p = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(p, __builtin_bit_cast(bf16x2, w0), scale, false);
+        p = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(p, __builtin_bit_cast(bf16x2, w1), scale, true);
+    } else {
+        p = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(p, __builtin_bit_cast(bf16x2, w0), scale, false);
+        p = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(p, __builtin_bit_cast(bf16x2, w1), scale, true);
+    }
+    return __builtin_bit_cast(uint32_t, p);
+}
+__device__ __forceinline__ uint32_t quick_codes4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float scale) {
+    uint32_t p = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(bf16x2, w0), scale, 0);
+    p = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(p, __builtin_bit_cast(bf16x2, w1), scale, 1);
+    p = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(p, __builtin_bit_cast(bf16x2, w2), scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(p, __builtin_bit_cast(bf16x2, w3), scale, 3);
+}
+// Quantizes and stores the chunk `c` of a block that a quad holds; returns the block's scale byte.
+template <int F> __device__ __forceinline__ uint32_t quantize_chunk(uint8_t* payload, int64_t c, uint4 v, bool store) {
+    if constexpr (Wire<F>::bits != 6) {
+        const QuickScale<F> q(group_umax(octet_amax_bits(v), 4));
+        if (q.ok) {                                              // uniform over the quad
+            if constexpr (F == FMT_E2M1) {
+                const uint32_t codes = quick_codes4(v.x, v.y, v.z, v.w, q.value());
+                if (store) *reinterpret_cast<uint32_t*>(payload + c * 4) = codes;
+            } else {
+                const uint2 codes = make_uint2(quick_codes8<F>(v.x, v.y, q.value()), quick_codes8<F>(v.z, v.w, q.value()));
+                if (store) *reinterpret_cast<uint2*>(payload + c * 8) = codes;
+            }
+            return q.byte;
+        }
+    }
+    const int e8 = wire_e8<F>(block_amax<F>(v));
+    emit_chunk<F>(payload, c, v, e8, store);
+    return (uint32_t)(127 - e8);
+}
+// the scale bytes of 4 consecutive blocks (16 lanes), in the first of the lanes
+__device__ __forceinline__ uint32_t gather_scales(uint32_t sb) {
+    constexpr int SHL4 = 0x104, SHL8 = 0x108, SHL12 = 0x10C;     // row_shl: lane i reads lane i + 4, 8, 12 of its 16
+    return sb | (dpp_u<SHL4>(sb) << 8) | (dpp_u<SHL8>(sb) << 16) | (dpp_u<SHL12>(sb) << 24);
+}
+
 // ------------------------------------------------------------------------------------------------
 // blocks of 32 along rows; the tensor is a flat array of 16-byte chunks (cols % 32 == 0)
 template <int F, int NV>
@@ -201,11 +264,8 @@ __global__ __launch_bounds__(WWG) void k_mx_quantize(const uint4* in, uint8_t* p
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int64_t c = base + k * WWG;
-        const int e8 = wire_e8<F>(block_amax<F>(v[k]));
-        emit_chunk<F>(payload, c, v[k], e8, c < nchunks);
         // the scale bytes of 4 consecutive blocks (16 lanes) leave as one 32-bit store
-        const uint32_t sb = (uint32_t)(127 - e8);
-        const uint32_t s4 = sb | (__shfl_down(sb, 4, 16) << 8) | (__shfl_down(sb, 8, 16) << 16) | (__shfl_down(sb, 12, 16) << 24);
+        const uint32_t s4 = gather_scales(quantize_chunk<F>(payload, c, v[k], c < nchunks));
         if (c < nchunks && (c & 15) == 0) {
             if (c + 16 <= nchunks) *reinterpret_cast<uint32_t*>(scales + (c >> 2)) = s4;
             else
@@ -315,11 +375,8 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int ch = k * DT + tid, r = ch >> 4, cc = ch & 15;
-        const int e8 = wire_e8<FR>(block_amax<FR>(v[k]));
         const int64_t cidx = (R0 + r) * row_chunks + (C0 >> 3) + cc;       // chunk index in the row-major payload
-        emit_chunk<FR>(row_payload, cidx, v[k], e8, ok[k]);
-        const uint32_t sb = (uint32_t)(127 - e8);
-        const uint32_t s4 = sb | (__shfl_down(sb, 4, 16) << 8) | (__shfl_down(sb, 8, 16) << 16) | (__shfl_down(sb, 12, 16) << 24);
+        const uint32_t sb = quantize_chunk<FR>(row_payload, cidx, v[k], ok[k]), s4 = gather_scales(sb);
         if (dword_row_scales && cols_valid == TILE_C) {
             if (ok[k] && cc == 0) *reinterpret_cast<uint32_t*>(row_scales + (cidx >> 2)) = s4;
         } else if (ok[k] && (cc & 3) == 0) row_scales[cidx >> 2] = (uint8_t)sb;
@@ -329,9 +386,32 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
 #pragma unroll
     for (int h = 0; h < BPT; ++h) {
         const int rb = (tid >> 7) * BPT + h;
+        uint8_t* dst = codes + c * CODE_PITCH + rb * blk_bytes;
+        if constexpr (Wire<FC>::bits != 6) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc_amax_pk(m, w[h][i]);
+            const QuickScale<FC> quick(amax_bits_of(m));
+            if (quick.ok) {
+                const float scale = quick.value();
+                s_cscale[c * 4 + rb] = (uint8_t)quick.byte;
+                if constexpr (FC == FMT_E2M1) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) q[i] = quick_codes4(w[h][4 * i], w[h][4 * i + 1], w[h][4 * i + 2], w[h][4 * i + 3], scale);
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+                } else {
+                    uint32_t q[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) q[i] = quick_codes8<FC>(w[h][2 * i], w[h][2 * i + 1], scale);
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+                    *reinterpret_cast<uint4*>(dst + 16) = make_uint4(q[4], q[5], q[6], q[7]);
+                }
+                continue;
+            }
+        }
         const int e8 = wire_e8<FC>(words_amax<FC>(w[h]));
         s_cscale[c * 4 + rb] = (uint8_t)(127 - e8);
-        uint8_t* dst = codes + c * CODE_PITCH + rb * blk_bytes;
         if constexpr (Fmt<FC>::hw) {
             uint32_t q[8];
 #pragma unroll
