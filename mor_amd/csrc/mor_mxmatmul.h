@@ -181,26 +181,41 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
 
     // step -> buffer; rows past the operand's end repeat its last one (their results are not stored), columns past k are 0
     constexpr int J = JA + JB;
-    auto copy_piece = [&](const uint8_t* ba, const uint8_t* bb, int buf, int j) {
-        if (j < JA) copy16_to_lds(lds0 + buf * STAGE + j * (NT * 16), ba, off_a[j < JA ? j : 0]);
-        else copy16_to_lds(lds0 + buf * STAGE + A_BYTES + (j - JA) * (NT * 16), bb, off_b[j >= JA ? j - JA : 0]);
+    auto copy_piece = [&](const uint8_t* ba, const uint8_t* bb, int slot, int j) {
+        if (j < JA) copy16_to_lds(lds0 + slot * STAGE + j * (NT * 16), ba, off_a[j < JA ? j : 0]);
+        else copy16_to_lds(lds0 + slot * STAGE + A_BYTES + (j - JA) * (NT * 16), bb, off_b[j >= JA ? j - JA : 0]);
     };
-    auto fetch = [&](int step, int buf) {
+    auto fetch = [&](int step, int slot) {
         const int s = step0 + step;
         if ((int64_t)(s + 1) * KS <= p.k) {
             const uint8_t *ba = scalar(ga + (int64_t)s * RA), *bb = scalar(gb + (int64_t)s * RB);
 #pragma unroll
-            for (int j = 0; j < J; ++j) copy_piece(ba, bb, buf, j);
+            for (int j = 0; j < J; ++j) copy_piece(ba, bb, slot, j);
         } else {
+            // (four loads at a time, in no branch of their own: a load in a branch is waited for before the next is issued)
+            constexpr int AT_ONCE = 4;
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const bool of_a = j < JA;
-                const int i = (of_a ? j : j - JA) * NT + tid;
-                const int c = of_a ? (i % CA) ^ swizzle<CA>(i / CA) : (i % CB) ^ swizzle<CB>(i / CB);
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (of_a ? s * RA + c * 16 < pitch_a : s * RB + c * 16 < pitch_b)
-                    v = *reinterpret_cast<const uint4*>(of_a ? ga + (int64_t)s * RA + off_a[of_a ? j : 0] : gb + (int64_t)s * RB + off_b[of_a ? 0 : j - JA]);
-                *reinterpret_cast<uint4*>(lds + buf * STAGE + (of_a ? 0 : A_BYTES) + i * 16) = v;
+            for (int j0 = 0; j0 < J; j0 += AT_ONCE) {
+                v4i v[AT_ONCE];
+                bool in[AT_ONCE];
+#pragma unroll
+                for (int e = 0; e < AT_ONCE; ++e) {
+                    const int j = j0 + e;
+                    if (j >= J) continue;
+                    const bool of_a = j < JA;
+                    const int i = (of_a ? j : j - JA) * NT + tid;
+                    const int c = of_a ? (i % CA) ^ swizzle<CA>(i / CA) : (i % CB) ^ swizzle<CB>(i / CB);
+                    in[e] = of_a ? s * RA + c * 16 < pitch_a : s * RB + c * 16 < pitch_b;
+                    const uint8_t* from = of_a ? ga + (in[e] ? (int64_t)s * RA + off_a[of_a ? j : 0] : 0) : gb + (in[e] ? (int64_t)s * RB + off_b[of_a ? 0 : j - JA] : 0);
+                    v[e] = *reinterpret_cast<const v4i*>(from);
+                }
+#pragma unroll
+                for (int e = 0; e < AT_ONCE; ++e) {
+                    const int j = j0 + e;
+                    if (j >= J) continue;
+                    const int i = (j < JA ? j : j - JA) * NT + tid;
+                    *reinterpret_cast<v4i*>(lds + slot * STAGE + (j < JA ? 0 : A_BYTES) + i * 16) = in[e] ? v[e] : v4i{0, 0, 0, 0};
+                }
             }
         }
     };
@@ -252,7 +267,7 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
     int sa[SM], sb[SN];
     uint2 raw_a[SM], raw_b[SN];
 
-    // One 16-byte read of the operands of depth u of the step in a buf: the reads of a depth are issued between the products
+    // One 16-byte read of the operands of depth u of the step in a slot: the reads of a depth are issued between the products
     // of the one before it, in the order in which its own products need them (B's first rows, A's, the rest of B's).
     constexpr int PA = BA == 8 ? 2 : 1, PB = BB == 8 ? 2 : 1;      // reads per 32 rows
     constexpr int READS = SM * PA + SN * PB;
@@ -265,20 +280,20 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
         else if (half == 0) f.lo = v;
         else f.hi = v;
     };
-    auto read_piece = [&](int buf, int u, int n) {
-        const uint8_t *base_a = lds + buf * STAGE + wm * RA, *base_b = lds + buf * STAGE + A_BYTES + wn * RB;
+    auto read_piece = [&](int slot, int u, int n) {
+        const uint8_t *base_a = lds + slot * STAGE + wm * RA, *base_b = lds + slot * STAGE + A_BYTES + wn * RB;
         if (n < PB) read_one(Int<CB>(), fb[u & 1][0], base_b, 0, u, n);
         else if (n < PB + SM * PA) read_one(Int<CA>(), fa[u & 1][(n - PB) / PA], base_a, (n - PB) / PA, u, (n - PB) % PA);
         else read_one(Int<CB>(), fb[u & 1][(n - SM * PA) / PB], base_b, (n - SM * PA) / PB, u, (n - SM * PA) % PB);
     };
-    auto read_codes = [&](int buf, int u) {
+    auto read_codes = [&](int slot, int u) {
 #pragma unroll
-        for (int n = 0; n < READS; ++n) read_piece(buf, u, n);
+        for (int n = 0; n < READS; ++n) read_piece(slot, u, n);
     };
-    auto spread_reads = [&](int buf, int u, int product) {
+    auto spread_reads = [&](int slot, int u, int product) {
         constexpr int SLOTS = SM * SN - SM, EACH = (READS + SLOTS - 1) / SLOTS;
 #pragma unroll
-        for (int n = product * EACH; n < (product + 1) * EACH && n < READS; ++n) read_piece(buf, u, n);
+        for (int n = product * EACH; n < (product + 1) * EACH && n < READS; ++n) read_piece(slot, u, n);
     };
     auto read_scales = [&](int step) {
         const uint8_t* base = s_scale + ((step / SS) & 1) * (2 * T * 16) + (step % SS) * NB;
@@ -323,10 +338,10 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
                 else asm volatile("" : "+v"(acc[i][j]));
             }
     };
-    auto inner_depths = [&](int buf) {
+    auto inner_depths = [&](int slot) {
         unroll<SUB - 1>([&](auto u) {
             constexpr int U = decltype(u)::value;
-            multiply(u, [&](int i) { spread_reads(buf, U + 1, i); __builtin_amdgcn_sched_barrier(0); });
+            multiply(u, [&](int i) { spread_reads(slot, U + 1, i); __builtin_amdgcn_sched_barrier(0); });
         });
     };
 
@@ -348,18 +363,18 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
     for (; group + 1 < whole; ++group) {                                 // no branch in here: all that is fetched is whole
 #pragma unroll
         for (int t = 0; t < SS; ++t) {
-            const int buf = t & 1;
+            const int slot = t & 1;
             if (t == 0) fetch_scales(group + 1, std::true_type());
-            inner_depths(buf);
+            inner_depths(slot);
             if (t == SS - 1) store_scales(group + 1);
             wait_and_sync();
             read_scales(group * SS + t + 1);
             __builtin_amdgcn_sched_barrier(0);
             multiply(Int<SUB - 1>(), [&](int i) {
                 constexpr int EACH = (J + SM * SN - 1) / (SM * SN);
-                spread_reads(buf ^ 1, 0, i);
+                spread_reads(slot ^ 1, 0, i);
 #pragma unroll
-                for (int j = i * EACH; j < (i + 1) * EACH && j < J; ++j) copy_piece(next_a, next_b, buf, j);
+                for (int j = i * EACH; j < (i + 1) * EACH && j < J; ++j) copy_piece(next_a, next_b, slot, j);
                 __builtin_amdgcn_sched_barrier(0);
             });
             next_a += RA;
@@ -367,16 +382,42 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
             take_scales();
         }
     }
+    if (nsteps == (group + 1) * SS && whole > group) {                   // the last group, where no ragged one follows
+#pragma unroll
+        for (int t = 0; t < SS; ++t) {
+            inner_depths(t & 1);
+            if (t + 1 < SS) {
+                wait_and_sync();
+                read_scales(group * SS + t + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            multiply(Int<SUB - 1>(), [&](int i) {
+                if (t + 1 < SS) {
+                    spread_reads((t & 1) ^ 1, 0, i);
+                    if (t + 2 < SS) {
+                        constexpr int EACH = (J + SM * SN - 1) / (SM * SN);
+#pragma unroll
+                        for (int j = i * EACH; j < (i + 1) * EACH && j < J; ++j) copy_piece(next_a, next_b, t & 1, j);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            next_a += RA;
+            next_b += RB;
+            if (t + 1 < SS) take_scales();
+        }
+        ++group;
+    }
     for (int s = group * SS; s < nsteps; ++s) {                          // the last whole group and a ragged one
-        const int buf = s & 1;
+        const int slot = s & 1;
         if (s % SS == 0 && s / SS + 1 < groups) fetch_scales(s / SS + 1, std::false_type());
-        inner_depths(buf);
+        inner_depths(slot);
         pin();
         if (s + 1 < nsteps) {
             if (s % SS == SS - 1) store_scales(s / SS + 1);
             wait_and_sync();
-            if (s + 2 < nsteps) fetch(s + 2, buf);
-            read_codes(buf ^ 1, 0);
+            if (s + 2 < nsteps) fetch(s + 2, slot);
+            read_codes(slot ^ 1, 0);
             read_scales(s + 1);
         }
         multiply(Int<SUB - 1>(), nothing);
@@ -463,11 +504,20 @@ template <int BITS> __device__ __forceinline__ Codes<BITS> codes128(const uint8_
         return f;
     }
 }
-// bytes g, 4 + g, 8 + g, 12 + g of 16 scale bytes
-__device__ __forceinline__ int scales_of_lane(uint4 v, int g) {
-    const uint32_t pick = 0x0C0C0400u + 0x0101u * g;                                   // byte g of either word
-    const uint32_t lo = __builtin_amdgcn_perm(v.y, v.x, pick), hi = __builtin_amdgcn_perm(v.w, v.z, pick);
-    return (int)(lo | (hi << 16));
+// scale bytes b + g, b + 4 + g, b + 8 + g and b + 12 + g of a row of nb, 0 past its end
+__device__ __forceinline__ int scales_of_lane(const uint8_t* row, int b, int nb, int g) {
+    if (b + 16 <= nb) {
+        const uint4 v = load16_any(row + b);
+        const uint32_t pick = 0x0C0C0400u + 0x0101u * g;                               // byte g of either word
+        const uint32_t lo = __builtin_amdgcn_perm(v.y, v.x, pick), hi = __builtin_amdgcn_perm(v.w, v.z, pick);
+        return (int)(lo | (hi << 16));
+    }
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = row[min(b + 4 * i + g, nb - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = b + 4 * i + g < nb ? e[i] : 0u;
+    return (int)(e[0] | (e[1] << 8) | (e[2] << 16) | (e[3] << 24));
 }
 
 template <int FA, int FB, int MT>
@@ -494,13 +544,13 @@ __global__ __launch_bounds__(512) void k_mx_skinny(const MxArgs p, int k_per_wav
         Codes<BB> fb[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) fb[c] = codes128<BB>(gb, k0 + 128 * c, pitch_b, g);
-        const int sb = scales_of_lane(scales16<true>(gsb, k0 / 32, nblocks), g);
+        const int sb = scales_of_lane(gsb, k0 / 32, nblocks, g);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             Codes<BA> fa[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) fa[c] = codes128<BA>(ga[i], k0 + 128 * c, pitch_a, g);
-            const int sa = scales_of_lane(scales16<true>(gsa[i], k0 / 32, nblocks), g);
+            const int sa = scales_of_lane(gsa[i], k0 / 32, nblocks, g);
             acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[0]), operand(fa[0]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 0, sb, 0, sa);
             acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[1]), operand(fa[1]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 1, sb, 1, sa);
             acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[2]), operand(fa[2]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 2, sb, 2, sa);
