@@ -267,10 +267,11 @@ MOR_API int mor_mx_dequantize(const void* payload, const void* scales, void* out
  * rounded to nearest even once.  The instructions add eight neighbouring products at a time, cut to 2^-14
  * of the largest one's power of two: products of two 4-bit codes lose nothing by that, the others the low
  * bits of small ones (at most 4.3e-4 of the sum of magnitudes, some 1e-5 as a rule).  A NaN code or a scale byte of 255 makes its row or column NaN.
- * k a positive multiple of 32 below 2^23; m and n positive, below 2^31; payloads 16-byte, output 2-byte
+ * k a positive multiple of 32 below 2^23; m and n positive, below 2^30, m * n at most 2^35; payloads 16-byte, output 2-byte
  * aligned.  Every result depends on the operands and the shape alone (no atomics).
- * The workspace (mor_mx_matmul_workspace_bytes, 0 for most shapes) holds fp32 partial sums of products
- * with few rows and columns, whose k is split; 16-byte aligned, not shared by calls that overlap.
+ * The workspace (mor_mx_matmul_workspace_bytes) holds the scale bytes of large products in the order in
+ * which the kernel reads them, or the fp32 partial sums of products with few rows and columns, whose k is
+ * split; 16-byte aligned, not shared by calls that overlap, NULL where its size is 0.
  */
 MOR_API size_t mor_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt);
 MOR_API int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_fmt, const void* b_payload,
@@ -286,7 +287,7 @@ MOR_API int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_fmt
  * or a NaN has scale byte 255 and comes back as NaNs.
  * gate and up: rows of cols contiguous elements, gate_stride / up_stride elements from row to row
  * (>= cols; the halves of one projection); output contiguous.  All four code and scale pointers NULL:
- * nothing is kept.  codes 8-byte, bf16 tensors 2-byte aligned; rows * ceil(cols / 32) < 2^30.
+ * nothing is kept.  codes 8-byte, bf16 tensors 2-byte aligned; rows * ceil(cols / 32) <= 2^30 - 64.
  */
 MOR_API int mor_swiglu_mx(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, void* output,
                           void* gate_codes, void* gate_scales, void* up_codes, void* up_scales,

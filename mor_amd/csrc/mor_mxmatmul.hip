@@ -50,8 +50,9 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt) {
     q.splits = 1;
     // Up to 32 rows of A: bound by reading B once (64 rows of A on 4096 x 4096 in E4M3: 23 us there, 14 us in tiles).  Four
     // waves share k where there are 512 workgroups and more (one row on 14336 x 4096 in E4M3: 16.0 us, with eight 19.4),
-    // eight where there are fewer (4096 x 14336 in E2M1: 8.6 us, with four 9.7).
-    if (m <= 32) {
+    // eight where there are fewer (4096 x 14336 in E2M1: 8.6 us, with four 9.7).  (From 2^28 columns on the grid would have
+    // 2^32 threads.)
+    if (m <= 32 && n < (1ll << 28)) {
         const int64_t pieces = cdiv(k, 512);                       // the loop's unit
         q.waves = (int)std::min<int64_t>(cdiv(n, 16) >= 512 ? 4 : 8, pieces);
         q.k_per_wave = (int)(cdiv(pieces, q.waves) * 512);
@@ -108,7 +109,8 @@ static int launch(MxArgs args, int a_fmt, int b_fmt, const MxPlan& q, hipStream_
 
 static bool product_format(int fmt) { return fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E5M2 || fmt == MOR_FMT_E2M1; }
 static bool product_shape(int64_t m, int64_t n, int64_t k) {
-    return m > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 23) && m < (1ll << 31) && n < (1ll << 31) && m <= MOR_MAX_ELEMENTS / n;      // (fewer than 2^25 tiles)
+    // a grid has fewer than 2^32 threads: 512 to 256 x 256 results, at most 2^22 tiles long
+    return m > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 23) && m < (1ll << 30) && n < (1ll << 30) && m <= MOR_MAX_ELEMENTS / n;
 }
 
 }  // namespace mor
@@ -126,7 +128,7 @@ extern "C" int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_
     if (!product_format(a_fmt) || !product_format(b_fmt))
         return mor_fail(MOR_ERR_INVALID_ARGUMENT, "products take the formats E4M3, E5M2 and E2M1 (got %d and %d)", a_fmt, b_fmt);
     if (!product_shape(m, n, k))
-        return mor_fail(MOR_ERR_INVALID_ARGUMENT, "products need k a positive multiple of 32 below 2^23, m and n positive and below 2^31, m * n at most 2^35 (got m %lld, n %lld, k %lld)",
+        return mor_fail(MOR_ERR_INVALID_ARGUMENT, "products need k a positive multiple of 32 below 2^23, m and n positive and below 2^30, m * n at most 2^35 (got m %lld, n %lld, k %lld)",
                         (long long)m, (long long)n, (long long)k);
     if ((reinterpret_cast<uintptr_t>(a_payload) | reinterpret_cast<uintptr_t>(b_payload)) & 15u)
         return mor_fail(MOR_ERR_INVALID_ARGUMENT, "payloads must be 16-byte aligned");

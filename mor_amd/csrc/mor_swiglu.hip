@@ -19,7 +19,8 @@ namespace mor {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi}); }
 
-// 1 / (1 + exp(-x)); exp and the reciprocal are the one-ulp instructions, far inside bf16's half step of 2^-9
+// 1 / (1 + exp(-x)); exp and the reciprocal are the one-ulp instructions, far inside bf16's half step of 2^-9 of a value.
+// Below x = -87.3, where it is under 2^-126, it may come out as 0.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x)); }
 
 struct SwigluShape {
@@ -138,7 +139,8 @@ using namespace mor;
 static int swiglu_shape(int64_t rows, int64_t cols, SwigluShape& sh) {
     if (rows <= 0 || cols <= 0) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "rows and cols must be positive (got %lld x %lld)", (long long)rows, (long long)cols);
     const int64_t blocks = cdiv(cols, 32);
-    if (blocks >= (1ll << 30) || rows > ((1ll << 30) - 1) / blocks) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "tensor too large (2^30 blocks of 32 or more)");
+    const int64_t most = (1ll << 30) - 64;                                   // a grid has fewer than 2^32 threads, four to a block
+    if (blocks > most || rows > most / blocks) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "tensor too large (more than 2^30 - 64 blocks of 32)");
     sh = SwigluShape{rows, cols, (uint32_t)(rows * blocks * 4), make_div((uint32_t)(blocks * 4))};
     return MOR_OK;
 }

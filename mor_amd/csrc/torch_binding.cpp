@@ -1,13 +1,14 @@
-// C++ registrations of the 14 `mor` operators for the CUDA dispatch key (which HIP tensors use under ROCm): the host
-// launchers of the reference (mor/csrc/cuda/fake_quantize.cu, "FQ": fake_quantize_cuda :1839-1871, _no_alloc
-// :1876-1907, quant_dequant / e4m3_with_e8_scale :1909-2011, block scaling :2013-2230, e8mx :2232-2397, channel
-// scaling :2431-2660, TORCH_LIBRARY_IMPL :2663-2678) rewritten as checks + allocations + one call into the C ABI of
-// libmor_hip.so.  The schemas are defined by mor_amd/ops.py; this file only provides faster implementations than
+// C++ registrations of the `mor` operators (the reference's 14, and those on the MX wire format at the end) for the CUDA
+// dispatch key (which HIP tensors use under ROCm): the host launchers of the reference (mor/csrc/cuda/fake_quantize.cu,
+// "FQ": fake_quantize_cuda :1839-1871, _no_alloc :1876-1907, quant_dequant / e4m3_with_e8_scale :1909-2011, block scaling
+// :2013-2230, e8mx :2232-2397, channel scaling :2431-2660, TORCH_LIBRARY_IMPL :2663-2678) rewritten as checks +
+// allocations + one call into the C ABI of libmor_hip.so.  The schemas are defined by mor_amd/ops.py; this file only provides faster implementations than
 // the Python ones (a few microseconds per call instead of ~14).  It contains no kernels and no arithmetic.
 #include <torch/library.h>
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
 
@@ -334,6 +335,9 @@ std::tuple<at::Tensor, at::Tensor> linear_forward(const at::Tensor& input, const
     const at::Tensor x = wire_input(input, "x"), w = wire_input(weight, "weight");
     const c10::OptionalDeviceGuard guard(x.device());
     const int64_t tokens = x.size(0), inputs = x.size(1), outputs = w.size(0);
+    // (each of them is the summed axis of a product: refused here rather than in the backward pass)
+    TORCH_CHECK((!keep_x || tokens <= (1 << 23) - 32) && inputs < (1 << 23) && outputs < (1 << 23),
+                "mor: at most 2^23 - 32 tokens, inputs and outputs, got ", tokens, ", ", inputs, " and ", outputs);
     const auto u8 = x.options().dtype(at::kByte);
     Parts scratch;
     const CodesAt xr = CodesAt::in(scratch, tokens, inputs, fmt), wr = CodesAt::in(scratch, outputs, inputs, fmt);
@@ -383,6 +387,24 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int6
     return std::get<0>(call_linear(x, w, fmt, false, false));
 }
 
+// A leaf's gradient is added on the stream that its live graphs were built on.  Where one was built on the default stream,
+// a backward pass under capture would have that stream wait for the captured one, which cannot be captured and ends the
+// process: refused while nothing is captured yet.  (Graphs built on another stream join the capture and leave it again.)
+void check_capture(const at::Tensor& t) {
+    if (!t.requires_grad() || !t.is_cuda() || t.key_set().has(c10::DispatchKey::Python)) return;      // (fake tensors)
+    const auto current = c10::hip::getCurrentHIPStream(t.device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    std::shared_ptr<torch::autograd::Node> node = t.grad_fn();
+    if (!node) node = torch::autograd::impl::try_get_grad_accumulator(t);
+    while (node && node->num_outputs() == 1) node = node->next_edge(0).function;            // views of a leaf
+    if (!node || !dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) return;
+    const auto stream = node->stream();
+    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
+                "mor: a graph built on the default stream holds a leaf of this call, whose backward pass cannot be captured then; "
+                "free that graph first, or build it on the capturing or another side stream");
+}
+
 // The quantisers are passed straight through.
 struct MxLinear : public torch::autograd::Function<MxLinear> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt,
@@ -416,6 +438,8 @@ at::Tensor mx_linear_autograd(const at::Tensor& x, const at::Tensor& w, int64_t 
         at::AutoDispatchBelowADInplaceOrView below;
         return std::get<0>(call_linear(x, w, fmt, false, false));
     }
+    check_capture(x);
+    check_capture(w);
     return MxLinear::apply(x, w, fmt, grad_fmt, need_x, need_w);
 }
 
@@ -444,6 +468,8 @@ at::Tensor swiglu_autograd(const at::Tensor& gate, const at::Tensor& up) {
         at::AutoDispatchBelowADInplaceOrView below;
         return std::get<0>(call_swiglu(gate, up, false));
     }
+    check_capture(gate);
+    check_capture(up);
     return SwigluMx::apply(gate, up);
 }
 

@@ -22,7 +22,7 @@ def linear(x: Tensor, weight: Tensor, fmt: int = wire.E4M3, grad_fmt: int = wire
         dw = Q(dy^T) Q(x^T)^T,     x^T in E4M3 whatever fmt is, blocks along the tokens (the last one filled up with zeros)
     x^T and weight^T are quantised in the forward pass, from the same read as their other orientation, and are all that
     is kept of x and weight: 1.03 bytes per element of x.  inputs and outputs are multiples of 32, the number of tokens
-    is any, zero included.  There is no second derivative."""
+    is any up to 2^23 - 32, zero included.  There is no second derivative."""
     if x.dim() == 2:
         return _op.mx_linear(x, weight, fmt, grad_fmt)
     if x.dim() < 2:

@@ -169,6 +169,19 @@ def test_captured_and_replayed(shape):
         assert torch.equal(outs[which], want), i
 
 
+def test_more_columns_than_the_few_row_kernel_has_threads_for():
+    """2^28 + 17 rows of B: offsets and a grid past 32 bits.  Rows of B repeat with a period, so the results do too."""
+    from mor_amd import wire
+    rng = np.random.default_rng(12)
+    n, period = 2 ** 28 + 17, 4099
+    (pa, sa), (pb, sb) = dev(*operand(rng, 1, 32, P.E2M1, 2)), dev(*operand(rng, period, 32, P.E2M1, 2))
+    times = -(-n // period)
+    got = wire.matmul_mx(pa, sa, pb.repeat(times, 1)[:n], sb.repeat(times, 1)[:n], wire.E2M1)
+    want = wire.matmul_mx(pa, sa, pb, sb, wire.E2M1)
+    whole = n // period * period
+    assert got.shape == (1, n) and (got[0, :whole].view(-1, period) == want).all() and torch.equal(got[0, whole:], want[0, : n - whole])
+
+
 def test_two_streams_at_once():
     from mor_amd import wire
     rng = np.random.default_rng(10)

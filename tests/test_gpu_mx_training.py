@@ -101,6 +101,18 @@ def test_linear_without_tokens():
     assert y.shape == (0, 32) and dx.shape == (0, 64) and dw.shape == (32, 64) and (dw == 0).all()
 
 
+def test_linear_token_limit():
+    """The weight's gradient sums over the tokens, of which a product takes fewer than 2^23: more are refused when they
+    come in, not when the gradient is asked for; without that gradient they are rows like any others."""
+    from mor_amd import mx
+    x, w = torch.zeros(2 ** 23, 32, dtype=torch.bfloat16, device="cuda"), leaf(randn(33, 32, 32))
+    x[-1] = 1
+    with pytest.raises(RuntimeError, match="tokens"):
+        mx.linear(x, w)
+    y = mx.linear(x, w.detach())
+    assert y.shape == (2 ** 23, 32) and (y[:-1] == 0).all() and torch.equal(y[-1:], mx.linear(x[-1:], w.detach()))
+
+
 def test_linear_keeps_its_activation_in_8_bits():
     from mor_amd import mx, wire
     kept = []
@@ -288,6 +300,34 @@ def test_training_step_captured_and_replayed():
         eager = step(*inputs[i])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(outs, want[i], eager)), i
+
+
+def test_capture_beside_a_live_eager_graph():
+    """Torch adds a leaf's gradient on the stream of the graph that holds it, and the default stream cannot join a capture:
+    the call is refused under capture while such a graph lives, and captured once it is freed."""
+    from mor_amd import mx
+    x, w = leaf(randn(84, 64, 64)), leaf(randn(85, 96, 64))
+    deep = leaf(randn(86, 2, 3, 64))
+    dh = randn(87, 64, 96).cuda()
+    want = torch.autograd.grad(mx.swiglu(mx.linear(x, w), mx.linear(x, w)), (x, w), dh)
+    for alive, calls in ((lambda: mx.linear(x, w), (lambda: mx.linear(x, w.detach()), lambda: mx.linear(x.detach(), w), lambda: mx.swiglu(x, x))),
+                         (lambda: mx.swiglu(deep, deep), (lambda: mx.linear(deep, w), lambda: mx.swiglu(deep.detach(), deep)))):
+        held = alive()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            for call in calls:
+                with pytest.raises(RuntimeError, match="default stream"):
+                    call()
+            with torch.no_grad():
+                calls[0]()
+        del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(mx.swiglu(mx.linear(x, w), mx.linear(x, w)), (x, w), dh)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_gradients_on_another_stream():

@@ -26,7 +26,7 @@ def test_product_refuses():
     for f in (2, 3, 5, -1):
         refused(call(fa=f), "formats")
         refused(call(fb=f), "formats")
-    for kw in (dict(k=0), dict(k=48), dict(k=-32), dict(k=1 << 23), dict(m=0), dict(m=-1), dict(n=0), dict(m=1 << 31), dict(m=1 << 30, n=1 << 30)):
+    for kw in (dict(k=0), dict(k=48), dict(k=-32), dict(k=1 << 23), dict(m=0), dict(m=-1), dict(n=0), dict(m=1 << 30), dict(n=1 << 30), dict(m=1 << 31), dict(m=1 << 29, n=1 << 29)):
         refused(call(**kw), "products need")
     refused(call(pa=A + 8), "16-byte")
     refused(call(pb=A + 4), "16-byte")
@@ -69,6 +69,7 @@ def test_swiglu_refuses():
     refused(call(us=0), "strides")
     refused(call(g=A + 1), "2-byte")
     refused(call(gc=A + 4), "8-byte")
+    refused(call(rows=(1 << 30) - 63, cols=32), "too large")
     refused(call(rows=1 << 29, cols=96, gs=96, us=96), "too large")
     refused(call(rows=1 << 62, cols=1 << 40, gs=1 << 40, us=1 << 40), "too large")
 
