@@ -127,6 +127,17 @@ template <int N, int I = 0, class F> __device__ __forceinline__ void unroll(F&& 
     }
 }
 
+// T x T results per workgroup, in steps of 128 bytes of every row; fp32 sums in registers throughout.
+//   T = 256: one workgroup per CU.  8-bit codes: four waves of 128 x 128 results, 256 accumulators a lane (with eight
+//   waves of 128 x 64 the operands spill or it is no faster); two 4-bit operands: eight waves (16384 x 14336 x 4096: 468 us,
+//   four waves 499), since their products are twice as fast and one wave per SIMD leaves them waiting.
+//   T = 128: four waves, two workgroups per CU, which cover each other's barriers.
+//   Steps of 128 bytes in two buffers; 64 bytes in four are slower (8192^3 E4M3: 450 -> 497 us): 128-byte rows are whole
+//   memory lines.
+// Bound by: 8-bit codes, the matrix units' power: 4096 x 4096 x 14336 E4M3 takes 186 us = 2.6 PFLOP/s with the units busy
+// 78 % of the cycles at the 2.2 GHz that the chip then holds (products alone 123 us, copies alone 180).  4-bit codes, LDS
+// beside them: a step's 2048 cycles of products read 196 KB and copy 64 KB in (2030 cycles): 16384 x 14336 x 4096 takes
+// 450 us = 4.3 PFLOP/s, 51 % busy.  A last round that fills half the CUs costs 3 %, not 12: the others clock higher.
 template <int FA, int FB, int T, int W>
 __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxArgs p) {
     constexpr int BA = Mx<FA>::bits, BB = Mx<FB>::bits;
@@ -490,7 +501,9 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
 // Up to 16 MT rows of A.  A workgroup owns 16 rows of B (columns of the output); its waves share k, each with its own
 // part, and add their sums through LDS in wave order.  Per 128 columns a wave reads 16 rows x 64 or 128 bytes of codes
 // straight into the operands of V_MFMA_SCALE_F32_16X16X128 (lane l = 16 g + r, row r: 4-bit columns 32 g .., 8-bit
-// columns 16 g .. and 64 + 16 g ..; scale of columns 32 g .. from lane 16 g + r).
+// columns 16 g .. and 64 + 16 g ..; scale of columns 32 g .. from lane 16 g + r).  Bound by reading B once: one row on
+// 14336 x 4096 in E2M1, 31 MB, takes 8.5 us with its launch (3.7 TB/s); holding the next 512 columns in registers meanwhile
+// made it 9.0 -> 10.8, non-temporal loads 9.7.
 template <int BITS> __device__ __forceinline__ Codes<BITS> codes128(const uint8_t* row, int k0, int pitch, int g) {
     const v4i zero = {0, 0, 0, 0};
     const int at = (BITS == 4 ? k0 / 2 : k0) + 16 * g;

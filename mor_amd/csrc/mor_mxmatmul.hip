@@ -8,7 +8,8 @@ namespace mor {
 
 // Scale bytes [rows, blocks] -> [groups of 16 blocks][rows][16], zeros past the last block.  A tile's 256 rows then have a
 // group's bytes in 4 KB that lie together; as the operands have them they are 16 bytes of each of 256 lines, a fifth of all
-// the lines that k_mx_tile would fetch.
+// the lines that k_mx_tile would fetch (4096 x 4096 x 14336 E4M3: 203 us without this kernel, 195 with it).  Bound by latency:
+// 5 us for 16384 + 14336 rows of k = 4096.
 __global__ __launch_bounds__(256) void k_mx_scales(const MxOperand a, const MxOperand b, uint4* out_a, uint4* out_b, int nblocks, int groups) {
     const MxOperand& o = blockIdx.y ? b : a;
     uint4* out = blockIdx.y ? out_b : out_a;
@@ -22,7 +23,8 @@ __global__ __launch_bounds__(256) void k_mx_scales(const MxOperand a, const MxOp
     }
 }
 
-// partial [splits][count] -> bf16, added in the order of the splits
+// partial [splits][count] -> bf16, added in fp32 in the order of the splits, whatever order they were computed in: the
+// result does not depend on the launch.  Bound by latency (3 us) at the sizes whose k is split.
 __global__ __launch_bounds__(256) void k_mx_join(const float* partial, uint16_t* out, int64_t count, int splits) {
     const int64_t step = (int64_t)gridDim.x * 256 * 4;
     const bool vec = (count & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;

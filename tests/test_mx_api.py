@@ -50,6 +50,8 @@ def test_quantisers_refuse():
     refused(L.mor_mx_quantize_dual_ragged(A, A, A, A, A, 0, 64, 4, 4, None), "positive")
     for pair in ((0, 4), (4, 1), (2, 2), (0, 1)):
         refused(L.mor_mx_quantize_dual_ragged(A, A, A, A, A, 33, 64, *pair, None), "formats")
+    refused(L.mor_mx_quantize_dual_ragged(A, A, A, A, A, 1 << 30, 32, 4, 4, None), "too many tiles")
+    refused(L.mor_mx_quantize_dual(A, A, A, A, A, 1 << 30, 32, 4, None), "too many tiles")
     refused(L.mor_mx_quantize_dual_ragged(A, A + 8, A, A, A, 33, 64, 4, 4, None), "aligned")
     refused(L.mor_selftest_hw_fp4(None, None), "NULL")
     assert L.mor_mx_payload_bytes(64, 128, 4) == 64 * 64
