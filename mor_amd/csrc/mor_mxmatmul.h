@@ -114,9 +114,9 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-// Where piece c of a row lies among the row's CH 16-byte pieces in LDS: 16 consecutive rows, read at the same c, cover the
-// 64 banks once (FP8 8192^3: 474 -> 450 us against an order that does so for 8 rows).
-template <int CH> __device__ __forceinline__ int swizzle(int row) { return CH == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
+// Where piece c of a row lies among the row's CH 16-byte pieces in LDS (c ^ swizzle): 16 consecutive rows, read at the same
+// c, cover the 64 banks once (FP8 8192^3: 474 -> 450 us against an order that does so for 8 rows).
+template <int CH> __device__ __forceinline__ int swizzle(int row) { return CH == 16 ? (row & 15) : CH == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
 
 template <int V> using Int = std::integral_constant<int, V>;
 // f(Int<0>()), ..., f(Int<N - 1>())
@@ -127,21 +127,23 @@ template <int N, int I = 0, class F> __device__ __forceinline__ void unroll(F&& 
     }
 }
 
-// T x T results per workgroup, in steps of 128 bytes of every row; fp32 sums in registers throughout.
-//   T = 256: one workgroup per CU.  8-bit codes: four waves of 128 x 128 results, 256 accumulators a lane (with eight
-//   waves of 128 x 64 the operands spill or it is no faster); two 4-bit operands: eight waves (16384 x 14336 x 4096: 468 us,
-//   four waves 499), since their products are twice as fast and one wave per SIMD leaves them waiting.
-//   T = 128: four waves, two workgroups per CU, which cover each other's barriers.
-//   Steps of 128 bytes in two buffers; 64 bytes in four are slower (8192^3 E4M3: 450 -> 497 us): 128-byte rows are whole
-//   memory lines.
+// T x T results per workgroup, in steps of KS columns of k in two buffers; fp32 sums in registers throughout.
+//   T = 256: steps of 128 bytes of the wider operand, one workgroup per CU.  8-bit codes: four waves of 128 x 128 results,
+//   256 accumulators a lane (with eight waves of 128 x 64 the operands spill or it is no faster); two 4-bit operands: eight
+//   waves (16384 x 14336 x 4096: 468 us, four waves 499), since their products are twice as fast and one wave per SIMD
+//   leaves them waiting.  64 bytes in four buffers are slower (8192^3 E4M3: 450 -> 497 us): 128-byte rows are whole lines.
+//   T = 128, four waves: the same steps, two workgroups per CU, which cover each other's barriers.
+//   T = 128, eight waves, and T = 64, two workgroups per CU: for results that do not fill the chip with larger tiles.  A step
+//   waits for its copies there, so it is twice as long, 256 columns: 1024 x 4096 x 4096 E4M3 22 us against 26 in four waves
+//   and short steps, 512 x 4096 x 4096 17 us (T = 64) against 23.5, 197 x 4127 x 2080 E4M3 x E2M1 9.6 against 13.4.
 // Bound by: 8-bit codes, the matrix units' power: 4096 x 4096 x 14336 E4M3 takes 186 us = 2.6 PFLOP/s with the units busy
 // 78 % of the cycles at the 2.2 GHz that the chip then holds (products alone 123 us, copies alone 180).  4-bit codes, LDS
 // beside them: a step's 2048 cycles of products read 196 KB and copy 64 KB in (2030 cycles): 16384 x 14336 x 4096 takes
 // 450 us = 4.3 PFLOP/s, 51 % busy.  A last round that fills half the CUs costs 3 %, not 12: the others clock higher.
 template <int FA, int FB, int T, int W>
-__global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxArgs p) {
+__global__ __launch_bounds__(W * 64, T == 256 || W == 8 ? 1 : 2) void k_mx_tile(const MxArgs p) {
     constexpr int BA = Mx<FA>::bits, BB = Mx<FB>::bits;
-    constexpr int KS = (BA == 4 && BB == 4) ? 256 : 128;           // columns of k per step: 128 bytes of the wider operand
+    constexpr int KS = (BA == 4 && BB == 4) || T == 64 || (T == 128 && W == 8) ? 256 : 128;
     constexpr int RA = KS * BA / 8, RB = KS * BB / 8;              // bytes per row and step
     constexpr int CA = RA / 16, CB = RB / 16;
     constexpr int SUB = KS / 64;                                   // matrix instructions' depths per step
@@ -151,10 +153,11 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
     constexpr int SM = T / 64, SN = T / (16 * W);                  // 32 x 32 results per wave: along m, along n
     constexpr int A_BYTES = T * RA, STAGE = T * (RA + RB);
     constexpr int JA = T * RA / (16 * NT), JB = T * RB / (16 * NT);          // 16-byte pieces per thread and step
-    constexpr int SR = 2 * T / NT;                                // rows whose scales a thread fetches
+    constexpr int SR = (2 * T + NT - 1) / NT;                      // rows whose scales a thread fetches
+    constexpr int SCALES = SR * NT * 16;                           // bytes of a group's scales: A's rows, B's, and repeats of the last
     constexpr int HIGH = SM * 32, WIDE = SN * 32, PITCH = WIDE * 2 + 16;    // a wave's results: rows, columns, bytes per row in LDS
-    __shared__ __attribute__((aligned(128))) uint8_t lds[std::max(2 * STAGE + 2 * 2 * T * 16, W * HIGH * PITCH)];
-    uint8_t* const s_scale = lds + 2 * STAGE;                      // [2][2 T rows: A's, then B's][16]
+    __shared__ __attribute__((aligned(128))) uint8_t lds[std::max(2 * STAGE + 2 * SCALES, W * HIGH * PITCH)];
+    uint8_t* const s_scale = lds + 2 * STAGE;                      // [2][A's rows, then B's][16]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
             const int g = step0 / SS + group;
 #pragma unroll
             for (int i = 0; i < SR; ++i)
-                copy16_to_lds(scales0 + (group & 1) * (2 * T * 16) + i * (NT * 16), scale_row[i] + g * (i * NT + wave * 64 < T ? stride_a : stride_b));
+                copy16_to_lds(scales0 + (group & 1) * SCALES + i * (NT * 16), scale_row[i] + g * (i * NT + wave * 64 < T ? stride_a : stride_b));
         } else {
             const int b = step0 * NB + group * 16;
 #pragma unroll
@@ -260,7 +263,7 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
     auto store_scales = [&](int group) {
         if constexpr (T != 256) {
 #pragma unroll
-            for (int i = 0; i < SR; ++i) *reinterpret_cast<uint4*>(s_scale + (group & 1) * (2 * T * 16) + (i * NT + tid) * 16) = held[i];
+            for (int i = 0; i < SR; ++i) *reinterpret_cast<uint4*>(s_scale + (group & 1) * SCALES + (i * NT + tid) * 16) = held[i];
         }
     };
 
@@ -302,12 +305,12 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
         for (int n = 0; n < READS; ++n) read_piece(slot, u, n);
     };
     auto spread_reads = [&](int slot, int u, int product) {
-        constexpr int SLOTS = SM * SN - SM, EACH = (READS + SLOTS - 1) / SLOTS;
+        constexpr int SLOTS = SM * SN > SM ? SM * SN - SM : 1, EACH = (READS + SLOTS - 1) / SLOTS;
 #pragma unroll
         for (int n = product * EACH; n < (product + 1) * EACH && n < READS; ++n) read_piece(slot, u, n);
     };
     auto read_scales = [&](int step) {
-        const uint8_t* base = s_scale + ((step / SS) & 1) * (2 * T * 16) + (step % SS) * NB;
+        const uint8_t* base = s_scale + ((step / SS) & 1) * SCALES + (step % SS) * NB;
         auto read = [&](const uint8_t* at) {
             if constexpr (NB == 8) return *reinterpret_cast<const uint2*>(at);
             else return make_uint2(*reinterpret_cast<const uint32_t*>(at), 0);
@@ -498,7 +501,7 @@ __global__ __launch_bounds__(W * 64, T == 256 ? 1 : 2) void k_mx_tile(const MxAr
     }
 }
 
-// Up to 16 MT rows of A.  A workgroup owns 16 rows of B (columns of the output); its waves share k, each with its own
+// Up to 16 rows of A.  A workgroup owns 16 rows of B (columns of the output); its waves share k, each with its own
 // part, and add their sums through LDS in wave order.  Per 128 columns a wave reads 16 rows x 64 or 128 bytes of codes
 // straight into the operands of V_MFMA_SCALE_F32_16X16X128 (lane l = 16 g + r, row r: 4-bit columns 32 g .., 8-bit
 // columns 16 g .. and 64 + 16 g ..; scale of columns 32 g .. from lane 16 g + r).  Bound by reading B once: one row on
@@ -533,87 +536,76 @@ __device__ __forceinline__ int scales_of_lane(const uint8_t* row, int b, int nb,
     return (int)(e[0] | (e[1] << 8) | (e[2] << 16) | (e[3] << 24));
 }
 
-template <int FA, int FB, int MT>
+template <int FA, int FB>
 __global__ __launch_bounds__(512) void k_mx_skinny(const MxArgs p, int k_per_wave) {
     constexpr int BA = Mx<FA>::bits, BB = Mx<FB>::bits;
-    extern __shared__ __attribute__((aligned(16))) float s_sum[];                      // [waves][MT][64 lanes][4]
+    extern __shared__ __attribute__((aligned(16))) float s_sum[];                      // [waves][64 lanes][4]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int r = lane & 15, g = lane >> 4;
     const int pitch_a = p.k / 8 * BA, pitch_b = p.k / 8 * BB, nblocks = p.k / 32;
     const int64_t n0 = (int64_t)blockIdx.x * 16, row_b = min(n0 + r, p.b.rows - 1);
     const uint8_t* gb = p.b.payload + row_b * pitch_b;
     const uint8_t* gsb = p.b.scales + row_b * nblocks;
-    const uint8_t *ga[MT], *gsa[MT];
-    v4f acc[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t row_a = min((int64_t)(16 * i + r), p.a.rows - 1);
-        ga[i] = p.a.payload + row_a * pitch_a;
-        gsa[i] = p.a.scales + row_a * nblocks;
-        acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    const int64_t row_a = min((int64_t)r, p.a.rows - 1);
+    const uint8_t* ga = p.a.payload + row_a * pitch_a;
+    const uint8_t* gsa = p.a.scales + row_a * nblocks;
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const int k_end = min(p.k, (wave + 1) * k_per_wave);
     for (int k0 = wave * k_per_wave; k0 < k_end; k0 += 512) {
         Codes<BB> fb[4];
+        Codes<BA> fa[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) fb[c] = codes128<BB>(gb, k0 + 128 * c, pitch_b, g);
         const int sb = scales_of_lane(gsb, k0 / 32, nblocks, g);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            Codes<BA> fa[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) fa[c] = codes128<BA>(ga[i], k0 + 128 * c, pitch_a, g);
-            const int sa = scales_of_lane(gsa[i], k0 / 32, nblocks, g);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[0]), operand(fa[0]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 0, sb, 0, sa);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[1]), operand(fa[1]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 1, sb, 1, sa);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[2]), operand(fa[2]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 2, sb, 2, sa);
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[3]), operand(fa[3]), acc[i], Mx<FB>::hw, Mx<FA>::hw, 3, sb, 3, sa);
-        }
+        for (int c = 0; c < 4; ++c) fa[c] = codes128<BA>(ga, k0 + 128 * c, pitch_a, g);
+        const int sa = scales_of_lane(gsa, k0 / 32, nblocks, g);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[0]), operand(fa[0]), acc, Mx<FB>::hw, Mx<FA>::hw, 0, sb, 0, sa);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[1]), operand(fa[1]), acc, Mx<FB>::hw, Mx<FA>::hw, 1, sb, 1, sa);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[2]), operand(fa[2]), acc, Mx<FB>::hw, Mx<FA>::hw, 2, sb, 2, sa);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(fb[3]), operand(fa[3]), acc, Mx<FB>::hw, Mx<FA>::hw, 3, sb, 3, sa);
     }
     v4f* sums = reinterpret_cast<v4f*>(s_sum);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sums[(wave * MT + i) * 64 + lane] = acc[i];
+    sums[wave * 64 + lane] = acc;
     __syncthreads();
-    // lane (g, r) of part i: row 16 i + r of the output, columns n0 + 4 g .. + 3
-    for (int t = threadIdx.x; t < MT * 64; t += blockDim.x) {
-        v4f v = sums[t];
-        for (int w = 1; w < waves; ++w) v += sums[w * MT * 64 + t];
-        const int64_t m = 16 * (t >> 6) + (t & 15), n = n0 + 4 * ((t >> 4) & 3);
-        if (m >= p.a.rows) continue;
-        uint16_t* at = p.out + m * p.out_stride + n;
-        const uint32_t lo = pack_bf16(v[0], v[1]), hi = pack_bf16(v[2], v[3]);
-        if (p.out16) {
-            if (n < p.b.rows) *reinterpret_cast<uint2*>(at) = make_uint2(lo, hi);
-        } else {
-            const uint16_t e[4] = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
+    if (wave) return;
+    // lane (g, r): row r of the output, columns n0 + 4 g .. + 3
+    v4f v = sums[lane];
+    for (int w = 1; w < waves; ++w) v += sums[w * 64 + lane];
+    const int64_t m = r, n = n0 + 4 * g;
+    if (m >= p.a.rows) return;
+    uint16_t* at = p.out + m * p.out_stride + n;
+    const uint32_t lo = pack_bf16(v[0], v[1]), hi = pack_bf16(v[2], v[3]);
+    if (p.out16) {
+        if (n < p.b.rows) *reinterpret_cast<uint2*>(at) = make_uint2(lo, hi);
+    } else {
+        const uint16_t e[4] = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < p.b.rows) at[j] = e[j];
-        }
+        for (int j = 0; j < 4; ++j)
+            if (n + j < p.b.rows) at[j] = e[j];
     }
 }
 
 // Which kernel, and how k is divided.
 struct MxPlan {
-    int tile;                      // k_mx_tile: 256 or 128; 0: k_mx_skinny
+    int tile;                      // k_mx_tile: 256, 128 or 64; 0: k_mx_skinny
+    int waves;                     // per workgroup
     int64_t cut_m, cut_n;          // tile 256: the rows and columns it takes, the rest in tiles of 128
     int splits, steps_per_split;   // k_mx_tile
-    int waves, k_per_wave;         // k_mx_skinny
+    int k_per_wave;                // k_mx_skinny
 };
 
 template <int FA, int FB> int launch_product(const MxArgs& args, const MxPlan& q, hipStream_t st) {
     if (q.tile == 0) {
-        const unsigned grid = (unsigned)cdiv(args.b.rows, 16), threads = q.waves * 64;
-        const int mt = args.a.rows <= 16 ? 1 : 2;
-        const size_t lds = (size_t)q.waves * mt * 1024;
-        if (mt == 1) k_mx_skinny<FA, FB, 1><<<grid, threads, lds, st>>>(args, q.k_per_wave);
-        else k_mx_skinny<FA, FB, 2><<<grid, threads, lds, st>>>(args, q.k_per_wave);
+        k_mx_skinny<FA, FB><<<(unsigned)cdiv(args.b.rows, 16), q.waves * 64, q.waves * 1024, st>>>(args, q.k_per_wave);
         return mor_check_launch("k_mx_skinny");
     }
     const dim3 grid((unsigned)(args.tiles_m * args.tiles_n), (unsigned)q.splits);
-    constexpr int W = Mx<FA>::bits == 4 && Mx<FB>::bits == 4 ? 8 : 4;
-    if (q.tile == 256) k_mx_tile<FA, FB, 256, W><<<grid, W * 64, 0, st>>>(args);
-    else k_mx_tile<FA, FB, 128, 4><<<grid, 256, 0, st>>>(args);
+    constexpr bool both4 = Mx<FA>::bits == 4 && Mx<FB>::bits == 4;
+    if (q.tile == 256) k_mx_tile<FA, FB, 256, both4 ? 8 : 4><<<grid, both4 ? 512 : 256, 0, st>>>(args);
+    else if (q.tile == 64) k_mx_tile<FA, FB, 64, 4><<<grid, 256, 0, st>>>(args);
+    else if (both4 || q.waves == 4) k_mx_tile<FA, FB, 128, 4><<<grid, 256, 0, st>>>(args);
+    else if constexpr (!both4) k_mx_tile<FA, FB, 128, 8><<<grid, 512, 0, st>>>(args);
     return mor_check_launch("k_mx_tile");
 }
 template <int FA> int launch_product(const MxArgs& args, int b_fmt, const MxPlan& q, hipStream_t st) {

@@ -47,49 +47,89 @@ __global__ __launch_bounds__(256) void k_mx_join(const float* partial, uint16_t*
 }
 
 static int bits_of(int fmt) { return fmt == MOR_FMT_E2M1 ? 4 : 8; }
+
+// Estimates in us, from the measurements below (operands of three calls in turn, in part from the last-level cache).
+//
+// Tiles of 128 or 64 and the parts that k is split into: 4 us, and a time per step that grows where two workgroups share a
+// CU's copies, but no less than the operands at 5 TB/s; for a split k 3 us more and 8 bytes per result and part at 4 TB/s.
+//   E4M3                      T = 64: whole, split     T = 128, eight waves     T = 128, four waves: whole, split
+//   1000 x 1000 x 1024             4.7, 10.8 in 2             7.3                       8.1
+//   512 x 4096 x 4096             16.9                       20.4                      23.5
+//   1024 x 4096 x 4096            30.6                       22.2                      25.7
+//   64 x 4096 x 4096              12.5, 10.0 in 4            19.0                      22.4, 12.5 in 4
+//   128 x 4096 x 14336            38.4, 20.6 in 4            64.1                      75.1, 22.8 in 8
+//   700 x 1000 x 14336            38.9, 29.8 in 2            64.0                      26.6 in 8
+//   64 x 65536 x 4096             66.7                                                 68.6              (T = 256: 85.1)
+//   128 x 65536 x 4096            94.7                                                 69.8              (T = 256: 84.2)
+// More tiles than run at once only where they are a single row or column: else the operands are read too often.
+static double small_tiles(MxPlan& q, int64_t m, int64_t n, int64_t k, int bits_a, int bits_b, bool split) {
+    const bool both4 = bits_a == 4 && bits_b == 4;
+    struct Shape { int tile, waves, columns, most; double us, shared; };           // us per step, and where all `most` run
+    const Shape shapes[] = {{64, 4, 256, 512, both4 ? 0.36 : 0.52, both4 ? 0.50 : 0.78}, {128, 8, 256, 256, 1.05, 1.05}, {128, 4, both4 ? 256 : 128, 512, 0.60, 0.60}};
+    const double operands = ((double)m * bits_a + (double)n * bits_b) * (double)k / 8.0 / 5.0e6;
+    double best = 1e30;
+    for (const Shape& s : shapes) {
+        const int64_t tiles = cdiv(m, s.tile) * cdiv(n, s.tile), steps = cdiv(k, s.columns), group = 512 / s.columns;
+        if (both4 && s.waves == 8) continue;
+        if (tiles > s.most && (std::min(m, n) > s.tile || s.waves == 8 || (s.tile == 64 && tiles >= (1ll << 22)))) continue;      // (2^32 threads)
+        const int64_t most = split ? std::max<int64_t>(1, std::min<int64_t>(s.most / tiles, steps / (2 * group))) : 1;
+        for (int64_t parts = 1; parts <= most; ++parts) {
+            const double over = std::min(1.0, std::max(0.0, (double)(tiles * parts - 256) / 256.0));
+            const double step = (s.us + over * (s.shared - s.us)) * (double)cdiv(tiles * parts, s.most);
+            const double us = 4.0 + std::max(operands, step * (double)cdiv(steps, parts)) +
+                              (parts > 1 ? 3.0 + (double)parts * (double)m * (double)n * 2e-6 : 0.0);
+            if (us >= best) continue;
+            best = us;
+            q.tile = s.tile;
+            q.waves = s.waves;
+            q.steps_per_split = (int)(cdiv(cdiv(steps, parts), group) * group);
+            q.splits = (int)cdiv(steps, q.steps_per_split);
+        }
+    }
+    return best;
+}
+// k_mx_skinny: 3 us, B at 5.6 TB/s and A, which every workgroup reads, at 12.
+//                                      m = 1     4       8      16    (tiles: 1 .. 16)
+//   m x 14336 x 4096 E2M1               8.6     9.2    10.0    11.7    10.3 .. 10.4
+//   m x 14336 x 4096 E4M3              13.6    14.6    16.0    19.0    13.6 .. 13.0
+//   m x 4096 x 14336 E4M3              13.3    13.8    14.2    16.7    16.8 .. 15.1
+//   m x 4096 x 4096 E4M3 x E2M1         4.0     4.4     4.8     5.5     6.3 .. 7.4
+//   m x 65536 x 4096 E4M3              50.0    54.3            72.8    62.0 .. 63.1  (from memory)
+static double few_rows(int64_t m, int64_t n, int64_t k, int bits_a, int bits_b) {
+    return 3.0 + (double)n * bits_b * (double)k / 8.0 / 5.6e6 + (double)(cdiv(n, 16) * m) * bits_a * (double)k / 8.0 / 12e6;
+}
+
 static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt) {
     MxPlan q{};
     q.splits = 1;
-    // Up to 32 rows of A: bound by reading B once (64 rows of A on 4096 x 4096 in E4M3: 23 us there, 14 us in tiles).  Four
-    // waves share k where there are 512 workgroups and more (one row on 14336 x 4096 in E4M3: 16.0 us, with eight 19.4),
-    // eight where there are fewer (4096 x 14336 in E2M1: 8.6 us, with four 9.7).  (From 2^28 columns on the grid would have
-    // 2^32 threads.)
-    if (m <= 32 && n < (1ll << 28)) {
+    const int bits_a = bits_of(a_fmt), bits_b = bits_of(b_fmt);
+    const int64_t large_m = cdiv(m, 256), large_n = cdiv(n, 256), large = large_m * large_n;
+    // Small tiles where they run in one round of 512, two to a CU (2560 x 4096 x 4096 in E4M3, 160 large tiles: 47 us, 55 in
+    // small ones; 2048 x 4096 x 4096, 128 of them: 46 us, 36 in small ones), or where large ones would be half empty.
+    if (large <= 128 || std::min(m, n) <= 128) {
+        const double us = small_tiles(q, m, n, k, bits_a, bits_b, true);
+        if (m > 16 || n >= (1ll << 28) || few_rows(m, n, k, bits_a, bits_b) >= us) return q;      // (a grid of 2^32 threads)
+        // Four waves share k where there are 512 workgroups and more (one row on 14336 x 4096 in E4M3: 16.0 us, with eight
+        // 19.4), eight where there are fewer (4096 x 14336 in E2M1: 8.6 us, with four 9.7).
         const int64_t pieces = cdiv(k, 512);                       // the loop's unit
+        q = MxPlan{};
+        q.splits = 1;
         q.waves = (int)std::min<int64_t>(cdiv(n, 16) >= 512 ? 4 : 8, pieces);
         q.k_per_wave = (int)(cdiv(pieces, q.waves) * 512);
         return q;
     }
-    const int ks = (bits_of(a_fmt) == 4 && bits_of(b_fmt) == 4) ? 256 : 128, group = 512 / ks;
-    const int64_t steps = cdiv(k, ks);
-    // 256 x 256 tiles where small ones would take more than one round of 512, two to a CU (2560 x 4096 x 4096 in E4M3, 160
-    // large tiles: 47 us, 55 in small ones; 2048 x 4096 x 4096, 128 of them: 46 us, 36 in small ones)
-    const int64_t large_m = cdiv(m, 256), large_n = cdiv(n, 256), large = large_m * large_n;
-    q.tile = large > 128 ? 256 : 128;
+    q.tile = 256;
+    q.steps_per_split = (int)(cdiv(k, 512) * (bits_a == 4 && bits_b == 4 ? 2 : 4));
     q.cut_m = m;
     q.cut_n = n;
     // A last round of large tiles on few CUs takes nearly as long as a full one: its columns or rows go to small tiles instead
-    // (4096 x 4608 x 4096 in E4M3, 288 tiles: 96 -> 82 us, 8192 x 4608, 576: 148 -> 137 us).  Of half a round that pays only
-    // after one full one (4096 x 6144, 384 tiles: 98 -> 95 us; 4096 x 14336, 896: 203 -> 209 us).
-    if (q.tile == 256 && large > 256) {
+    // (4096 x 4608 x 4096 in E4M3, 288 tiles: 96 -> 74 us, 8192 x 4608, 576: 148 -> 133 us).  Of half a round that pays only
+    // after one full one (4096 x 6144, 384 tiles: 98 -> 93 us; 4096 x 14336, 896: 203 -> 209 us).
+    if (large > 256) {
         const int64_t full = large / 256 * 256, most = large < 512 ? 128 : 64, c_n = full / large_m, c_m = full / large_n;
         if (large > full && large - c_n * large_m <= most) q.cut_n = std::min(n, c_n * 256);
         else if (large > full && large - c_m * large_n <= most) q.cut_m = std::min(m, c_m * 256);
     }
-    const int64_t tiles = cdiv(m, q.tile) * cdiv(n, q.tile);
-    // k is split where small tiles leave CUs idle, by the smallest of 4 us + 0.6 us a step (two workgroups share a CU
-    // without slowing each other: a step waits for memory) and, when split, 3 us + 8 bytes per result and part at 4 TB/s
-    // (128 x 4096 x 14336 in E4M3: 106 us whole, 28 us in 8 parts)
-    int64_t splits = 1;
-    if (q.tile == 128) {
-        double best = 1e30;
-        for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(512 / tiles, steps / (2 * group))); ++s) {
-            const double us = 0.6 * (double)cdiv(steps, s) + (s > 1 ? 3.0 + (double)s * (double)m * (double)n * 2e-6 : 0.0);
-            if (us < best) { best = us; splits = s; }
-        }
-    }
-    q.steps_per_split = (int)(cdiv(cdiv(steps, splits), group) * group);
-    q.splits = (int)cdiv(steps, q.steps_per_split);
     return q;
 }
 
@@ -168,8 +208,8 @@ extern "C" int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_
         if (int rc = mor_check_launch("k_mx_scales")) return rc;
         if (int rc = launch(args, a_fmt, b_fmt, q, st)) return rc;
         if (cut_m == m && cut_n == n) return MOR_OK;
-        MxPlan small = q;
-        small.tile = 128;
+        MxPlan small{};
+        small_tiles(small, rest.a.rows, rest.b.rows, k, bits_of(a_fmt), bits_of(b_fmt), false);
         return launch(rest, a_fmt, b_fmt, small, st);
     }
     if (need) args.partial = static_cast<float*>(workspace);

@@ -14,7 +14,8 @@ NAMES = {P.E4M3: "E4M3", P.E5M2: "E5M2", P.E2M1: "E2M1"}
 # tiles, steps and groups; k that is a multiple of 512, 128, 64 and 32; k split over workgroups
 SHAPES = [(1, 1, 32), (1, 16, 96), (3, 50, 512), (16, 33, 544), (17, 1000, 2080), (32, 4100, 1024), (33, 1, 64), (64, 130, 4096),
           (65, 33, 32), (100, 129, 160), (128, 128, 4096), (129, 257, 4160), (197, 1031, 1056), (513, 256, 14336), (1100, 1000, 320),
-          (3585, 3333, 96), (3840, 3328, 1056), (3584, 3600, 2048), (4096, 3584, 1664)]
+          (600, 4001, 352), (1100, 4008, 160), (61, 33000, 96), (33000, 120, 64),
+          (700, 1000, 14336), (3585, 3333, 96), (3840, 3328, 1056), (3584, 3600, 2048), (4096, 3584, 1664)]
 
 
 def ids(v):
