@@ -4,7 +4,8 @@ The reference's ops only return bf16 (mor/ops.py); these functions are the step 
 payload a scaled-MFMA GEMM consumes.  The quantization is the reference's MX block rule (block modes with sf_type 2,
 mor/csrc/cuda/fake_quantize.cu:801-823, :251-252): blocks of 32 elements, scale 2^floor(log2(fmax / amax)), so
 `dequantize_mx(*quantize_mx(x, fmt), fmt)` equals `mor.ops.fake_quantize(x, ..., 1, 32, 0.0, mode, 2)[0]` (mode 2 for
-E4M3, 3 for E5M2) wherever the latter's values are not the exponent-clamp artefacts of that kernel.
+E4M3, 3 for E5M2) wherever the latter's values are not the exponent-clamp artefacts of that kernel.  E2M1 (4-bit codes) and
+the product of two tensors in the wire format, matmul_mx, have no counterpart there.
 """
 from typing import Optional, Tuple
 
