@@ -93,6 +93,9 @@ template <bool SHORT> __device__ __forceinline__ uint4 scales16(const uint8_t* r
     return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
+// (m0 is reserved, which the compiler remarks on at every use of these; the clobber keeps its own settings of m0 apart)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes from memory to LDS without passing through registers: lane i's piece lands at lds + 16 i.  (The compiler does
 // not see the write, so it does not wait for it before unrelated LDS reads; every reader is behind wait_and_sync().)
 __device__ __forceinline__ void copy16_to_lds(uint32_t lds, const uint8_t* base, uint32_t offset) {
@@ -101,6 +104,7 @@ __device__ __forceinline__ void copy16_to_lds(uint32_t lds, const uint8_t* base,
 __device__ __forceinline__ void copy16_to_lds(uint32_t lds, const uint8_t* from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // a pointer that is the same in every lane, in scalar registers
 __device__ __forceinline__ const uint8_t* scalar(const uint8_t* p) {
     const uint64_t x = reinterpret_cast<uint64_t>(p);

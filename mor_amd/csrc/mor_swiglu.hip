@@ -6,7 +6,7 @@
 // Forward reads 4 and writes 2 + 2.0625 bytes per element, backward reads 2 + 2.0625 and writes 4.  A lane owns 8
 // consecutive elements of a row, a quad of lanes a block (k_swiglu_mx / k_swiglu_mx_backward); arithmetic in fp32, one
 // rounding to bf16 per result (bf16 is the tensors' type), the codes' rounding is the E4M3 grid's.
-// Bound by memory: 16384 x 14336 takes 320 us either way, 5.9 TB/s (a copy of that size reaches 4.9).  Rows that cannot be
+// Bound by memory: 16384 x 14336 takes 306 us either way, 6.2 TB/s (a 2 GiB copy reaches 4.9, a cold one of 128 MiB 6.2).  Rows that cannot be
 // read as aligned vectors go element by element, which the caches gather: 4096 x 14335 87 us, x 14336 82; whole chunks as
 // one access at a 2-byte address are no faster (86).
 
@@ -32,22 +32,34 @@ struct SwigluShape {
     DivU32 per_row;           // 8-element chunks per row: 4 ceil(cols / 32)
 };
 
-// 8 elements of a row from column c on, zeros past the end.  VEC: the row's chunks are 16-byte aligned and whole.
-template <bool VEC> __device__ __forceinline__ uint4 load8(const uint16_t* row, int64_t c, int64_t cols) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if constexpr (VEC) {
-        if (c < cols) v = *reinterpret_cast<const uint4*>(row + c);
-    } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = c + i < cols ? row[c + i] : 0u;
-        v = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
-    }
-    return v;
+// 8 elements from column c on of each of N rows, zeros past the end.  VEC: the rows' chunks are 16-byte aligned and whole.
+// Large tensors go past the caches: inputs and gradients beyond 2^25 elements, h beyond 2^26, codes beyond 2^27, where they
+// do not stay in the last-level cache until they are used.  Forward and the quantization of h after it: 4096 x 14336 127 ->
+// 113 us (117 with h past the caches), 16384 x 14336 537 -> 522; backward and two quantizations: 162 -> 159 and 749 -> 722;
+// of 2048 x 14336 57.7 -> 59.9 and 77 -> 83, so not there.  Codes: 16384 x 14336 forward 327 -> 307, 8192 x 14336 133 -> 153.
+__device__ __forceinline__ bool beyond(const SwigluShape& sh, int log2_elements) { return ((int64_t)sh.chunks * 8) >> log2_elements != 0; }
+__device__ __forceinline__ void store_codes(uint8_t* at, uint2 q, bool nt) {
+    if (nt) __builtin_nontemporal_store(((uint64_t)q.y << 32) | q.x, reinterpret_cast<uint64_t*>(at));
+    else *reinterpret_cast<uint2*>(at) = q;
 }
-template <bool VEC> __device__ __forceinline__ void store8(uint16_t* row, int64_t c, int64_t cols, uint4 v) {
+template <bool VEC, int N> __device__ __forceinline__ void load8(uint4 (&v)[N], const uint16_t* const (&row)[N], int64_t c, int64_t cols, bool nt) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = make_uint4(0, 0, 0, 0);
     if constexpr (VEC) {
-        if (c < cols) *reinterpret_cast<uint4*>(row + c) = v;
+        if (c < cols) load16_group(v, nt, [&](int k) { return reinterpret_cast<const uint4*>(row[k] + c); });
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            uint32_t e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = c + i < cols ? row[k][c + i] : 0u;
+            v[k] = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+        }
+    }
+}
+template <bool VEC> __device__ __forceinline__ void store8(uint16_t* row, int64_t c, int64_t cols, uint4 v, bool nt) {
+    if constexpr (VEC) {
+        if (c < cols) store16_rt(reinterpret_cast<uint4*>(row + c), v, nt);
     } else {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -92,14 +104,17 @@ __global__ __launch_bounds__(256) void k_swiglu_mx(const uint16_t* gate, int64_t
     const bool in = i < sh.chunks;                                           // whole quads
     const uint32_t row = div_u32(in ? i : 0u, sh.per_row);
     const int64_t c = in ? (int64_t)(i - row * sh.per_row.d) * 8 : sh.cols;
-    const uint4 g = load8<VEC>(gate + row * gate_stride, c, sh.cols), u = load8<VEC>(up + row * up_stride, c, sh.cols);
-    store8<VEC>(out + row * sh.cols, c, sh.cols, make_uint4(swiglu2(g.x, u.x), swiglu2(g.y, u.y), swiglu2(g.z, u.z), swiglu2(g.w, u.w)));
+    uint4 v[2];
+    load8<VEC>(v, {gate + row * gate_stride, up + row * up_stride}, c, sh.cols, beyond(sh, 25));
+    const uint4 g = v[0], u = v[1];
+    store8<VEC>(out + row * sh.cols, c, sh.cols, make_uint4(swiglu2(g.x, u.x), swiglu2(g.y, u.y), swiglu2(g.z, u.z), swiglu2(g.w, u.w)),
+                beyond(sh, 26));
     if constexpr (KEEP) {
         uint32_t sg, su;
         const uint2 qg = encode8(g, sg), qu = encode8(u, su);
         if (in) {
-            *reinterpret_cast<uint2*>(gate_codes + (int64_t)i * 8) = qg;
-            *reinterpret_cast<uint2*>(up_codes + (int64_t)i * 8) = qu;
+            store_codes(gate_codes + (int64_t)i * 8, qg, beyond(sh, 27));
+            store_codes(up_codes + (int64_t)i * 8, qu, beyond(sh, 27));
             if ((i & 3u) == 0) { gate_scales[i >> 2] = (uint8_t)sg; up_scales[i >> 2] = (uint8_t)su; }
         }
     }
@@ -113,7 +128,9 @@ __global__ __launch_bounds__(256) void k_swiglu_mx_backward(const uint16_t* grad
     if (i >= sh.chunks) return;
     const uint32_t row = div_u32(i, sh.per_row);
     const int64_t c = (int64_t)(i - row * sh.per_row.d) * 8;
-    const uint4 d = load8<VEC>(grad + row * sh.cols, c, sh.cols);
+    uint4 v[1];
+    load8<VEC>(v, {grad + row * sh.cols}, c, sh.cols, beyond(sh, 25));
+    const uint4 d = v[0];
     float g[8], u[8];
     decode8(*reinterpret_cast<const uint2*>(gate_codes + (int64_t)i * 8), gate_scales[i >> 2], g);
     decode8(*reinterpret_cast<const uint2*>(up_codes + (int64_t)i * 8), up_scales[i >> 2], u);
@@ -131,8 +148,8 @@ __global__ __launch_bounds__(256) void k_swiglu_mx_backward(const uint16_t* grad
         wg[k] = pack2(a[0], a[1]);
         wu[k] = pack2(b[0], b[1]);
     }
-    store8<VEC>(grad_gate + row * sh.cols, c, sh.cols, make_uint4(wg[0], wg[1], wg[2], wg[3]));
-    store8<VEC>(grad_up + row * sh.cols, c, sh.cols, make_uint4(wu[0], wu[1], wu[2], wu[3]));
+    store8<VEC>(grad_gate + row * sh.cols, c, sh.cols, make_uint4(wg[0], wg[1], wg[2], wg[3]), beyond(sh, 25));
+    store8<VEC>(grad_up + row * sh.cols, c, sh.cols, make_uint4(wu[0], wu[1], wu[2], wu[3]), beyond(sh, 25));
 }
 
 }  // namespace mor
