@@ -390,19 +390,26 @@ at::Tensor mx_linear(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int6
 // A leaf's gradient is added on the stream that its live graphs were built on.  Where one was built on the default stream,
 // a backward pass under capture would have that stream wait for the captured one, which cannot be captured and ends the
 // process: refused while nothing is captured yet.  (Graphs built on another stream join the capture and leave it again.)
-void check_capture(const at::Tensor& t) {
-    if (!t.requires_grad() || !t.is_cuda() || t.key_set().has(c10::DispatchKey::Python)) return;      // (fake tensors)
-    const auto current = c10::hip::getCurrentHIPStream(t.device().index());
+void check_capture(const at::Tensor& a, const at::Tensor& b) {
+    const int device = a.device().index();
+    if (!a.is_cuda() || a.key_set().has(c10::DispatchKey::Python)) return;                       // (fake tensors)
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
-    std::shared_ptr<torch::autograd::Node> node = t.grad_fn();
-    if (!node) node = torch::autograd::impl::try_get_grad_accumulator(t);
-    while (node && node->num_outputs() == 1) node = node->next_edge(0).function;            // views of a leaf
-    if (!node || !dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) return;
-    const auto stream = node->stream();
-    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
-                "mor: a graph built on the default stream holds a leaf of this call, whose backward pass cannot be captured then; "
-                "free that graph first, or build it on the capturing or another side stream");
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device).stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return;
+    }
+    if (status == hipStreamCaptureStatusNone) return;
+    for (const at::Tensor& t : {a, b}) {
+        if (!t.requires_grad()) continue;
+        std::shared_ptr<torch::autograd::Node> node = t.grad_fn();
+        if (!node) node = torch::autograd::impl::try_get_grad_accumulator(t);
+        while (node && node->num_outputs() == 1) node = node->next_edge(0).function;             // views of a leaf
+        if (!node || !dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) continue;
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(device).id(),
+                    "mor: a graph built on the default stream holds a leaf of this call, whose backward pass cannot be captured then; "
+                    "free that graph first, build it on a side stream, or, for a forward pass alone, call under torch.no_grad()");
+    }
 }
 
 // The quantisers are passed straight through.
@@ -438,8 +445,7 @@ at::Tensor mx_linear_autograd(const at::Tensor& x, const at::Tensor& w, int64_t 
         at::AutoDispatchBelowADInplaceOrView below;
         return std::get<0>(call_linear(x, w, fmt, false, false));
     }
-    check_capture(x);
-    check_capture(w);
+    check_capture(x, w);
     return MxLinear::apply(x, w, fmt, grad_fmt, need_x, need_w);
 }
 
@@ -468,8 +474,7 @@ at::Tensor swiglu_autograd(const at::Tensor& gate, const at::Tensor& up) {
         at::AutoDispatchBelowADInplaceOrView below;
         return std::get<0>(call_swiglu(gate, up, false));
     }
-    check_capture(gate);
-    check_capture(up);
+    check_capture(gate, up);
     return SwigluMx::apply(gate, up);
 }
 
