@@ -267,8 +267,8 @@ MOR_API int mor_mx_dequantize(const void* payload, const void* scales, void* out
  * rounded to nearest even once.  The instructions add eight neighbouring products at a time, cut to 2^-14
  * of the largest one's power of two: products of two 4-bit codes lose nothing by that, the others the low
  * bits of small ones (at most 4.3e-4 of the sum of magnitudes, some 1e-5 as a rule).  A NaN code or a scale byte of 255 makes its row or column NaN.
- * k a positive multiple of 32 below 2^23; m and n positive, below 2^30, m * n at most 2^35; payloads 16-byte, output 2-byte
- * aligned.  Every result depends on the operands and the shape alone (no atomics).
+ * k a positive multiple of 32 below 2^23; m and n positive, below 2^30, m * n at most 2^35; payloads 16-byte,
+ * output 2-byte aligned.  Every result depends on the operands and the shape alone (no atomics).
  * The workspace (mor_mx_matmul_workspace_bytes) holds the scale bytes of large products in the order in
  * which the kernel reads them, or the fp32 partial sums of products with few rows and columns, whose k is
  * split; 16-byte aligned, not shared by calls that overlap, NULL where its size is 0.

@@ -9,7 +9,7 @@
 //   4-bit codes: columns 32 h .. 32 h + 31;
 //   the scale of columns 32 h .. 32 h + 31 comes from lane 32 h + r.
 // B's rows go in as the instruction's first operand, so that a lane ends up with consecutive columns of the output.
-//   k_mx_tile    256 x 256 or 128 x 128 tiles of the output, both operands through LDS
+//   k_mx_tile    tiles of 256 x 256, 128 x 128 or 64 x 64 results, both operands through LDS
 //   k_mx_skinny  few rows of A: B's codes go from memory to the registers of the one wave that needs them
 //   k_mx_join    adds the partial sums of a k_mx_tile launch whose k was split
 
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(W * 64, T == 256 || W == 8 ? 1 : 2) void k_mx_tile(
         }
     };
     // scale bytes: 16 per row, i.e. SS steps, at a time.  T = 256: a group's lie together (k_mx_scales) and are copied like
-    // the codes; T = 128: straight from the operands, through registers
+    // the codes; smaller tiles: straight from the operands, through registers
     const uint8_t* scale_row[SR];
 #pragma unroll
     for (int i = 0; i < SR; ++i) {
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(W * 64, T == 256 || W == 8 ? 1 : 2) void k_mx_tile(
         }
     };
 
-    // this wave's quarter of the tile
+    // this wave's part of the tile
     const int wm = (wave / (W / 2)) * (32 * SM), wn = (wave % (W / 2)) * (32 * SN);
     v16f acc[SN][SM];                                                // [B's 32 rows][A's 32 rows]
 #pragma unroll

@@ -419,9 +419,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         at::AutoDispatchBelowADInplaceOrView below;
         auto [y, kept] = call_linear(x, w, fmt, need_w, need_x);
         ctx->save_for_backward({kept});
-        ctx->saved_data["fmts"] = fmt * 16 + grad_fmt;
-        ctx->saved_data["kept"] = (int64_t)need_w * 2 + (int64_t)need_x;
-        ctx->saved_data["inputs"] = w.size(1);
+        ctx->saved_data["call"] = w.size(1) << 8 | fmt << 4 | grad_fmt << 2 | (int64_t)need_w << 1 | (int64_t)need_x;      // (fmt 0 or 4, grad_fmt 0 or 1)
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -429,10 +427,11 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
         at::Tensor dx, dw;
         if (grads[0].defined()) {
             static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, int64_t, int64_t, int64_t, bool, bool)>("mor::mx_linear_backward");
-            const int64_t fmts = ctx->saved_data["fmts"].toInt(), kept = ctx->saved_data["kept"].toInt();
-            std::tie(dx, dw) = op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["inputs"].toInt(), fmts / 16, fmts % 16, kept & 2, kept & 1);
-            if (!(kept & 1)) dx = at::Tensor();
-            if (!(kept & 2)) dw = at::Tensor();
+            const int64_t call = ctx->saved_data["call"].toInt();
+            const bool need_w = call & 2, need_x = call & 1;
+            std::tie(dx, dw) = op.call(grads[0], ctx->get_saved_variables()[0], call >> 8, call >> 4 & 15, call >> 2 & 3, need_w, need_x);
+            if (!need_x) dx = at::Tensor();
+            if (!need_w) dw = at::Tensor();
         }
         return {dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     }
