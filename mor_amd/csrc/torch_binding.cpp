@@ -412,6 +412,13 @@ void check_capture(const at::Tensor& a, const at::Tensor& b) {
     }
 }
 
+// A tangent would be lost without a word: below the autograd key nothing carries one (torch.func.jvp, forward_ad; a dual
+// tensor need not require a gradient).
+void refuse_tangents(std::initializer_list<at::Tensor> inputs, const char* what) {
+    for (const at::Tensor& t : inputs)
+        TORCH_CHECK(!(t.defined() && t._fw_grad(0).defined()), "mor: ", what, " has no forward-mode derivative");
+}
+
 // The quantisers are passed straight through.
 struct MxLinear : public torch::autograd::Function<MxLinear> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt,
@@ -424,6 +431,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "mor: mx.linear has no second derivative");
+        refuse_tangents({grads[0]}, "the gradient of mx.linear");
         at::Tensor dx, dw;
         if (grads[0].defined()) {
             static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, int64_t, int64_t, int64_t, bool, bool)>("mor::mx_linear_backward");
@@ -439,6 +447,7 @@ struct MxLinear : public torch::autograd::Function<MxLinear> {
 
 at::Tensor mx_linear_autograd(const at::Tensor& x, const at::Tensor& w, int64_t fmt, int64_t grad_fmt) {
     check_grad_fmt(grad_fmt);
+    refuse_tangents({x, w}, "mx.linear");
     const bool on = at::GradMode::is_enabled(), need_x = on && x.requires_grad(), need_w = on && w.requires_grad();
     if (!need_x && !need_w) {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -461,6 +470,7 @@ struct SwigluMx : public torch::autograd::Function<SwigluMx> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "mor: mx.swiglu has no second derivative");
+        refuse_tangents({grads[0]}, "the gradient of mx.swiglu");
         if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
         static auto op = handle<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&)>("mor::swiglu_mx_backward");
         auto [dg, du] = op.call(grads[0], ctx->get_saved_variables()[0]);
@@ -469,6 +479,7 @@ struct SwigluMx : public torch::autograd::Function<SwigluMx> {
 };
 at::Tensor swiglu(const at::Tensor& gate, const at::Tensor& up) { return std::get<0>(call_swiglu(gate, up, false)); }
 at::Tensor swiglu_autograd(const at::Tensor& gate, const at::Tensor& up) {
+    refuse_tangents({gate, up}, "mx.swiglu");
     if (!at::GradMode::is_enabled() || !(gate.requires_grad() || up.requires_grad())) {
         at::AutoDispatchBelowADInplaceOrView below;
         return std::get<0>(call_swiglu(gate, up, false));

@@ -22,7 +22,7 @@ def linear(x: Tensor, weight: Tensor, fmt: int = wire.E4M3, grad_fmt: int = wire
         dw = Q(dy^T) Q(x^T)^T,     x^T in E4M3 whatever fmt is, blocks along the tokens (the last one filled up with zeros)
     x^T and weight^T are quantised in the forward pass, from the same read as their other orientation, and are all that
     is kept of x and weight: 1.03 bytes per element of x.  inputs and outputs are multiples of 32, the number of tokens
-    is any up to 2^23 - 32, zero included.  There is no second derivative."""
+    is any up to 2^23 - 32, zero included.  There is no second derivative and no forward-mode one: a call with a tangent is refused."""
     if x.dim() == 2:
         return _op.mx_linear(x, weight, fmt, grad_fmt)
     if x.dim() < 2:
@@ -36,7 +36,8 @@ def swiglu(gate: Tensor, up: Tensor) -> Tensor:
     For the backward pass gate and up are kept as E4M3 codes with a scale byte per 32 elements of a row, written by the
     forward kernel: 2.0625 bytes per pair of elements instead of 4 in bf16.  The gradients are
     those of the formula at the decoded values.  A block that holds an infinity or a NaN comes back as NaNs.  Rows may
-    lie at any stride (the halves of one projection are read in place).  There is no second derivative."""
+    lie at any stride (the halves of one projection are read in place).  There is no second derivative and no
+    forward-mode one: a call with a tangent is refused."""
     if gate.shape != up.shape:
         raise RuntimeError(f"mor: gate and up must have one shape, got {tuple(gate.shape)} and {tuple(up.shape)}")
     if gate.dim() == 2:
