@@ -254,7 +254,8 @@ MOR_API int mor_mx_quantize_dual(const void* input, void* row_payload, void* row
 MOR_API int mor_mx_quantize_dual_ragged(const void* input, void* row_payload, void* row_scales, void* col_payload,
                          void* col_scales, int64_t rows, int64_t cols, int row_fmt, int col_fmt, void* stream);
 
-/* payload + scales -> bf16 [rows, cols] (blocks of 32 along rows). */
+/* payload + scales -> bf16 [rows, cols] (blocks of 32 along rows).  A block with scale byte 255, the E8M0 NaN, decodes to
+ * NaNs in every format. */
 MOR_API int mor_mx_dequantize(const void* payload, const void* scales, void* output, int64_t rows,
                       int64_t cols, int fmt, void* stream);
 

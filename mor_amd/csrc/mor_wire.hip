@@ -652,7 +652,7 @@ __global__ __launch_bounds__(WWG) void k_mx_dequantize(const uint8_t* payload, c
                 continue;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = de == 128 ? u2f(0x7FC00000u) : fp4_value(q >> (4 * i));      // 128: the E8M0 NaN
+            for (int i = 0; i < 8; ++i) x[i] = fp4_value(q >> (4 * i));
         } else {
             if (fp6_decode_hw_ok(de)) {
                 // every lane of the quad reads its block's 24 bytes (same addresses: one fetch) and decodes all 32 codes
@@ -676,6 +676,10 @@ __global__ __launch_bounds__(WWG) void k_mx_dequantize(const uint8_t* payload, c
                 const uint32_t code = (uint32_t)(bits >> (6 * i)) & 0x3Fu;
                 x[i] = u2f(f2u(fp6_value<F>(code & 0x1Fu)) | ((code & 0x20u) << 26));
             }
+        }
+        if (de == 128) {                         // scale byte 255, the E8M0 NaN (the product takes it so too)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = u2f(0x7FC00000u);
         }
         uint4 r;
         r.x = store_pair<true>(ldexpf(x[0], de), ldexpf(x[1], de));

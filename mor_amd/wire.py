@@ -53,7 +53,7 @@ def quantize_mx_dual(x: Tensor, fmt: int = E4M3) -> Tuple[Tensor, Tensor, Tensor
 
 
 def dequantize_mx(payload: Tensor, scales: Tensor, fmt: int = E4M3) -> Tensor:
-    """payload + scales -> bf16 [rows, 32 * scales.shape[1]]"""
+    """payload + scales -> bf16 [rows, 32 * scales.shape[1]]; a block with scale byte 255 (the E8M0 NaN) is NaNs"""
     return _op.mx_dequantize(payload, scales, fmt)
 
 
