@@ -278,6 +278,11 @@ MOR_API size_t mor_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, in
 MOR_API int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_fmt, const void* b_payload,
                           const void* b_scales, int b_fmt, void* output, int64_t m, int64_t n, int64_t k,
                           void* workspace, size_t workspace_bytes, void* stream);
+/* Which kernels mor_mx_matmul runs for a product (for measurements and tests): plan[0], tile: 256, 128 or 64 results
+ * square, 0 for the kernel of up to 16 rows; plan[1], waves per workgroup; plan[2], parts of k; plan[3] and plan[4], the
+ * rows and columns of the first launch, plan[5] and plan[6], tile and waves of a second one for the others, 0 where there
+ * is none; plan[7], the most threads of a launch. */
+MOR_API int mor_mx_matmul_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int64_t* plan);
 
 /*
  * Gated activation that keeps its inputs in 8 bits (no counterpart in the reference):

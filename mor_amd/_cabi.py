@@ -43,6 +43,7 @@ SIGNATURES = {
     "mor_mx_quantize_dual": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "mor_mx_quantize_dual_ragged": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _vp]),
     "mor_mx_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
+    "mor_mx_matmul_plan": (_int, [_i64, _i64, _i64, _int, _int, _vp]),
     "mor_mx_matmul": (_int, [_vp, _vp, _int, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
     "mor_swiglu_mx": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "mor_swiglu_mx_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),

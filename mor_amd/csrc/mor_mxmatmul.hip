@@ -46,6 +46,9 @@ __global__ __launch_bounds__(256) void k_mx_join(const float* partial, uint16_t*
     }
 }
 
+// A grid has fewer than 2^32 threads: past that it is cut without an error.
+static bool fits_a_grid(int64_t workgroups, int waves) { return workgroups < (1ll << 32) / (waves * 64); }
+
 static int bits_of(int fmt) { return fmt == MOR_FMT_E2M1 ? 4 : 8; }
 
 // Estimates in us, from the measurements below (operands of three calls in turn, in part from the last-level cache).
@@ -71,7 +74,7 @@ static double small_tiles(MxPlan& q, int64_t m, int64_t n, int64_t k, int bits_a
     for (const Shape& s : shapes) {
         const int64_t tiles = cdiv(m, s.tile) * cdiv(n, s.tile), steps = cdiv(k, s.columns), group = 512 / s.columns;
         if (both4 && s.waves == 8) continue;
-        if (tiles > s.most && (std::min(m, n) > s.tile || s.waves == 8 || (s.tile == 64 && tiles >= (1ll << 22)))) continue;      // (2^32 threads)
+        if (tiles > s.most && (std::min(m, n) > s.tile || s.waves == 8 || !fits_a_grid(tiles, s.waves))) continue;
         const int64_t most = split ? std::max<int64_t>(1, std::min<int64_t>(s.most / tiles, steps / (2 * group))) : 1;
         for (int64_t parts = 1; parts <= most; ++parts) {
             const double over = std::min(1.0, std::max(0.0, (double)(tiles * parts - 256) / 256.0));
@@ -108,17 +111,19 @@ static MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt) {
     // small ones; 2048 x 4096 x 4096, 128 of them: 46 us, 36 in small ones), or where large ones would be half empty.
     if (large <= 128 || std::min(m, n) <= 128) {
         const double us = small_tiles(q, m, n, k, bits_a, bits_b, true);
-        if (m > 16 || n >= (1ll << 28) || few_rows(m, n, k, bits_a, bits_b) >= us) return q;      // (a grid of 2^32 threads)
         // Four waves share k where there are 512 workgroups and more (one row on 14336 x 4096 in E4M3: 16.0 us, with eight
         // 19.4), eight where there are fewer (4096 x 14336 in E2M1: 8.6 us, with four 9.7).
         const int64_t pieces = cdiv(k, 512);                       // the loop's unit
+        const int waves = (int)std::min<int64_t>(cdiv(n, 16) >= 512 ? 4 : 8, pieces);
+        if (m > 16 || !fits_a_grid(cdiv(n, 16), waves) || few_rows(m, n, k, bits_a, bits_b) >= us) return q;
         q = MxPlan{};
         q.splits = 1;
-        q.waves = (int)std::min<int64_t>(cdiv(n, 16) >= 512 ? 4 : 8, pieces);
+        q.waves = waves;
         q.k_per_wave = (int)(cdiv(pieces, q.waves) * 512);
         return q;
     }
     q.tile = 256;
+    q.waves = bits_a == 4 && bits_b == 4 ? 8 : 4;
     q.steps_per_split = (int)(cdiv(k, 512) * (bits_a == 4 && bits_b == 4 ? 2 : 4));
     q.cut_m = m;
     q.cut_n = n;
@@ -149,9 +154,16 @@ static int launch(MxArgs args, int a_fmt, int b_fmt, const MxPlan& q, hipStream_
                                                                                                    : launch_product_e2m1(args, b_fmt, q, st);
 }
 
+// what a cut last round leaves: rows or columns in small tiles
+static MxPlan rest_plan(const MxPlan& q, int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt) {
+    MxPlan r{};
+    small_tiles(r, q.cut_m < m ? m - q.cut_m : m, q.cut_n < n ? n - q.cut_n : n, k, bits_of(a_fmt), bits_of(b_fmt), false);
+    return r;
+}
+
 static bool product_format(int fmt) { return fmt == MOR_FMT_E4M3 || fmt == MOR_FMT_E5M2 || fmt == MOR_FMT_E2M1; }
 static bool product_shape(int64_t m, int64_t n, int64_t k) {
-    // a grid has fewer than 2^32 threads: 512 to 256 x 256 results, at most 2^22 tiles long
+    // (tiles of 128 by four waves fit a grid at any such size: m or n below 2^30 in one row or column of tiles is 2^31 threads)
     return m > 0 && n > 0 && k > 0 && k % 32 == 0 && k < (1ll << 23) && m < (1ll << 30) && n < (1ll << 30) && m <= MOR_MAX_ELEMENTS / n;
 }
 
@@ -162,6 +174,30 @@ using namespace mor;
 extern "C" size_t mor_mx_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt) {
     if (!product_shape(m, n, k) || !product_format(a_fmt) || !product_format(b_fmt)) return 0;
     return mx_workspace(mx_plan(m, n, k, a_fmt, b_fmt), m, n, k);
+}
+
+extern "C" int mor_mx_matmul_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int64_t* plan) {
+    if (!plan) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "plan is NULL");
+    if (!product_shape(m, n, k) || !product_format(a_fmt) || !product_format(b_fmt)) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "no such product");
+    const MxPlan q = mx_plan(m, n, k, a_fmt, b_fmt);
+    auto threads = [](const MxPlan& p, int64_t rows, int64_t cols) {
+        return (p.tile ? cdiv(rows, p.tile) * cdiv(cols, p.tile) : cdiv(cols, 16)) * p.waves * 64;      // along the grid's first axis
+    };
+    const bool large = q.tile == 256, cut = large && (q.cut_m < m || q.cut_n < n);
+    plan[0] = q.tile;
+    plan[1] = q.waves;
+    plan[2] = q.splits;
+    plan[3] = large ? q.cut_m : m;
+    plan[4] = large ? q.cut_n : n;
+    plan[5] = plan[6] = 0;
+    plan[7] = threads(q, plan[3], plan[4]);
+    if (cut) {
+        const MxPlan r = rest_plan(q, m, n, k, a_fmt, b_fmt);
+        plan[5] = r.tile;
+        plan[6] = r.waves;
+        plan[7] = std::max(plan[7], threads(r, q.cut_m < m ? m - q.cut_m : m, q.cut_n < n ? n - q.cut_n : n));
+    }
+    return MOR_OK;
 }
 
 extern "C" int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_fmt, const void* b_payload, const void* b_scales, int b_fmt,
@@ -208,9 +244,7 @@ extern "C" int mor_mx_matmul(const void* a_payload, const void* a_scales, int a_
         if (int rc = mor_check_launch("k_mx_scales")) return rc;
         if (int rc = launch(args, a_fmt, b_fmt, q, st)) return rc;
         if (cut_m == m && cut_n == n) return MOR_OK;
-        MxPlan small{};
-        small_tiles(small, rest.a.rows, rest.b.rows, k, bits_of(a_fmt), bits_of(b_fmt), false);
-        return launch(rest, a_fmt, b_fmt, small, st);
+        return launch(rest, a_fmt, b_fmt, rest_plan(q, m, n, k, a_fmt, b_fmt), st);
     }
     if (need) args.partial = static_cast<float*>(workspace);
     if (int rc = launch(args, a_fmt, b_fmt, q, st)) return rc;
