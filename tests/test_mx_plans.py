@@ -44,3 +44,28 @@ def test_the_few_row_kernel_ends_where_its_grid_does():
     assert at((1 << 28) - 16)["tile"] == 0 and at((1 << 28) - 16)["waves"] == 4
     for n in ((1 << 28) - 15, (1 << 28) - 1, 1 << 28):
         assert at(n)["tile"] != 0
+
+
+def kind(shape, pair):
+    """the kernels and launches of a product: widths of the codes, tile, waves, k split or not, what is cut, the rest's tiles"""
+    q = plan(*shape, *pair)
+    cut = "rows" if q["rows"] < shape[0] else "columns" if q["cols"] < shape[1] else ""
+    return ("4x4" if pair == (P.E2M1, P.E2M1) else "8x4" if P.E2M1 in pair else "8x8", q["tile"], q["waves"], q["parts"] > 1, cut, q["rest_tile"], q["rest_waves"])
+
+
+def test_every_kind_of_plan_is_among_the_tested_sizes():
+    """Plans of sizes drawn over the whole range, against those of the sizes that the GPU tests multiply exactly."""
+    import random
+    import test_gpu_mx_matmul as base
+    import test_gpu_mx_plans as more
+    # (the largest sizes of the older list run with three of the pairs)
+    few = ((P.E4M3, P.E4M3), (P.E2M1, P.E2M1), (P.E4M3, P.E2M1))
+    tested = {kind(s, p) for s in base.SHAPES for p in base.PAIRS if p in few or s[0] * s[1] <= 1 << 20} | {kind(s, p) for s, p in more.CASES}
+    rng = random.Random(20)
+    size = lambda top: round(2 ** rng.uniform(0, top))  # noqa: E731
+    drawn = {}
+    for _ in range(40000):
+        shape, pair = (size(16.1), size(16.1), 32 * size(9.3)), rng.choice(few)
+        drawn.setdefault(kind(shape, pair), shape)
+    missing = {k: s for k, s in drawn.items() if k not in tested}
+    assert len(drawn) > 40 and not missing, missing
