@@ -165,13 +165,18 @@ at::Tensor e8mx_autograd(const at::Tensor& input, int64_t dim_x, int64_t dim_y, 
 // The MX wire format and the operators on it (mor_amd/wire.py, mor_amd/mx.py; not in the reference)
 int64_t payload_bytes(int64_t n, int64_t fmt) { return (int64_t)mor_mx_payload_bytes(1, n, (int)fmt); }
 
-// A 2-D bf16 GPU tensor, contiguous and 16-byte aligned (a view that is not is copied)
+// contiguous and at a multiple of `bytes`: a view that is not is copied
+at::Tensor aligned(const at::Tensor& t, uintptr_t bytes) {
+    const at::Tensor x = t.contiguous();
+    return reinterpret_cast<uintptr_t>(x.data_ptr()) % bytes ? x.clone() : x;
+}
+
+// A 2-D bf16 GPU tensor, contiguous and 16-byte aligned
 at::Tensor wire_input(const at::Tensor& t, const char* what) {
     TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.is_cuda(), "mor: ", what, " must be a 2-D bfloat16 GPU tensor, got ",
                 t.scalar_type(), " ", t.sizes());
     TORCH_CHECK(t.size(1) > 0 && t.size(1) % 32 == 0, "mor: ", what, ": MX blocks need columns that are a multiple of 32, got ", t.sizes());
-    const at::Tensor x = t.contiguous();
-    return (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15u) ? x.clone() : x;
+    return aligned(t, 16);
 }
 
 std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor& input, int64_t fmt) {
@@ -205,7 +210,7 @@ at::Tensor mx_dequantize(const at::Tensor& payload, const at::Tensor& scales, in
     TORCH_CHECK(fmt >= MOR_FMT_E4M3 && fmt <= MOR_FMT_E2M1, "mor: unknown element format ", fmt);
     const int64_t rows = scales.size(0), cols = scales.size(1) * 32;
     TORCH_CHECK(payload.numel() == (cols ? rows * payload_bytes(cols, fmt) : 0), "mor: payload size does not match the scales");
-    const at::Tensor p = payload.contiguous(), s = scales.contiguous();
+    const at::Tensor p = aligned(payload, 16), s = aligned(scales, 4);
     const c10::OptionalDeviceGuard guard(p.device());
     at::Tensor out = at::empty({rows, cols}, p.options().dtype(at::kBFloat16));
     if (rows) check(mor_mx_dequantize(p.data_ptr(), s.data_ptr(), out.data_ptr(), rows, cols, (int)fmt, stream_of(p)));
@@ -224,7 +229,7 @@ at::Tensor mx_matmul(const at::Tensor& a, const at::Tensor& a_scales, const at::
     side(b, b_scales, b_fmt, "b");
     TORCH_CHECK(a.device() == b.device(), "mor: a and b must be on one device");
     TORCH_CHECK(a_scales.size(1) == b_scales.size(1), "mor: a and b must have the same number of columns, got ", a_scales.size(1) * 32, " and ", b_scales.size(1) * 32);
-    const at::Tensor pa = a.contiguous(), sa = a_scales.contiguous(), pb = b.contiguous(), sb = b_scales.contiguous();
+    const at::Tensor pa = aligned(a, 16), sa = a_scales.contiguous(), pb = aligned(b, 16), sb = b_scales.contiguous();
     const c10::OptionalDeviceGuard guard(pa.device());
     const int64_t m = pa.size(0), n = pb.size(0), k = sa.size(1) * 32;
     const auto options = pa.options().dtype(at::kBFloat16);
