@@ -282,11 +282,10 @@ __global__ __launch_bounds__(WWG) void k_mx_quantize(const uint4* in, uint8_t* p
 // ------------------------------------------------------------------------------------------------
 // both orientations from one read, blocks along rows in format FR, along columns in FC.  Tile 128 rows x 128 columns;
 // cols % 32 == 0.  Where rows % 32 != 0 the last block of every column is filled up with zeros.  Bound by memory, which
-// takes reads of 256-byte pieces and writes of 64 (E2M1) or 128 bytes per row and column worse than a copy: 8192 x 8192 in
-// E2M1 39 us (5.2 TB/s; read alone 23.6, without the transposed codes 36.7, without the codes along rows 37.7 of the 46
-// before the next two), E4M3 47 (5.8 TB/s).  So two workgroups per CU do better than four on tensors that come from memory
-// (see launch_dual), where their reads are also kept out of the caches.  Tiles of 256 rows (25 -> 32 us at 2080 x 14336) and the next tile's loads held in registers over the
-// column phase (24 -> 26) were slower.
+// takes reads of 256-byte pieces and writes of 64 (E2M1) or 128 bytes per row and column worse than a copy: 8192 x 8192 takes
+// 41.7 us in E2M1 with its input in memory and 32.8 with it in the last-level cache (4.9 and 6.2 TB/s), 52.5 and 41.6 in E4M3
+// (5.2 and 6.6 TB/s).  Two workgroups per CU do better than four on large tensors (see launch_dual).  Tiles of 256 rows (25 ->
+// 32 us at 2080 x 14336) and the next tile's loads held in registers over the column phase (24 -> 26) were slower.
 constexpr int TILE_C = 128;
 constexpr int TILE_ROWS = 128;
 constexpr int DUAL_THREADS = 512;
@@ -363,9 +362,10 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
     const bool full = rows_valid == TR && cols_valid == TILE_C;            // the same in every lane
     uint4 v[NV];
     if (full) {
-        // (beyond 2^25 elements nothing of the input is left in the last-level cache for a later call: 8192 x 8192 E4M3
-        // 52.4 -> 46.8 us, E2M1 41.5 -> 39.1; 4096 x 4096 11.8 -> 15.4)
-        load16_group(v, rows * cols > ((int64_t)1 << 25), [&](int k) { return in + first + k * step; });
+        // (plain loads: past the caches an input that is still in the last-level cache takes longer, 8192 x 8192 E4M3 41.6 ->
+        // 47.1 us, E2M3 42.0 -> 48.5, and one that is not no less, 52.5 -> 53.6 and 51.7 -> 51.0)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) v[k] = in[first + k * step];
     } else {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -834,8 +834,9 @@ static int launch_dual(const void* input, void* row_payload, void* row_scales, v
     const int64_t tiles_y = (rows + TILE_ROWS - 1) / TILE_ROWS, tiles_x = (cols + TILE_C - 1) / TILE_C;
     // (a grid of 2^32 threads would be cut without an error: one tile column of 2^30 rows)
     if (tiles_y * tiles_x >= (1ll << 32) / DUAL_THREADS) return mor_fail(MOR_ERR_INVALID_ARGUMENT, "too many tiles");
-    // From 2^25 elements on, LDS that is not used keeps a third workgroup off a CU (8192 x 8192 E2M1: 46.3 -> 41.7 us, E4M3
-    // 56.3 -> 52.1, 8192 x 14336 E2M1 85 -> 78; 4096 x 8192 22.6 and 22.5; below, 4096 x 4096, 10.6 -> 11.9 us).
+    // From 2^25 elements on, LDS that is not used keeps a third workgroup off a CU.  8192 x 8192, input in memory: E2M1 46.1 ->
+    // 41.7 us, E4M3 56.5 -> 52.3, E2M3 56.4 -> 51.7; in the last-level cache 33.6 -> 32.8, 42.0 -> 41.6, 41.5 -> 41.8; 16384 x
+    // 14336 E2M1 167 -> 145, E4M3 197 -> 190; 8192 x 4096 E4M3 30.3 -> 29.6 and 21.7 -> 22.8.  Below, 4096 x 4096, 10.6 -> 11.9.
     const unsigned spare = rows * cols >= ((int64_t)1 << 25) ? 40000u : 0u;
     k_mx_dual<FR, FC, TILE_ROWS, DUAL_THREADS><<<(unsigned)(tiles_y * tiles_x), DUAL_THREADS, spare, st>>>(
         static_cast<const uint4*>(input), static_cast<uint8_t*>(row_payload), static_cast<uint8_t*>(row_scales),
