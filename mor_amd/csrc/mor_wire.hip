@@ -333,9 +333,10 @@ static DualMap dual_tile_map(int64_t tiles_x, int64_t tiles_y) {
     return {0, make_div((uint32_t)tiles_x)};
 }
 
-template <int FR, int FC, int TR, int DT>
-__global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_payload, uint8_t* row_scales,
+template <int FR, int FC>
+__global__ __launch_bounds__(DUAL_THREADS) void k_mx_dual(const uint4* in, uint8_t* row_payload, uint8_t* row_scales,
                                                  uint8_t* col_payload, uint8_t* col_scales, int64_t rows, int64_t cols, DualMap map) {
+    constexpr int TR = TILE_ROWS, DT = DUAL_THREADS;
     constexpr int NV = TR * (TILE_C / 8) / DT;   // 16-byte chunks per thread
     constexpr int RB = TR / 32;                   // row blocks per tile column
     constexpr int BPT = TILE_C * RB / DT;        // column blocks per thread
@@ -345,7 +346,8 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
     constexpr int SEGS = RB * blk_bytes / SEG;    // per column
     // one buffer, two uses: the bf16 tile, then the codes of the column blocks (smaller)
     __shared__ __attribute__((aligned(16))) uint16_t tile[TR * TILE_C];
-    __shared__ __attribute__((aligned(4))) uint8_t s_cscale[TILE_C * 4];
+    static_assert(RB == 4, "the column blocks' scale bytes leave as one word");
+    __shared__ __attribute__((aligned(4))) uint8_t s_cscale[TILE_C * RB];
     uint8_t* codes = reinterpret_cast<uint8_t*>(tile);
     static_assert(TILE_C * CODE_PITCH <= TR * TILE_C * 2, "the code tile must fit the bf16 tile");
     const int tid = threadIdx.x;
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
             const QuickScale<FC> quick(amax_bits_of(m));
             if (quick.ok) {
                 const float scale = quick.value();
-                s_cscale[c * 4 + rb] = (uint8_t)quick.byte;
+                s_cscale[c * RB + rb] = (uint8_t)quick.byte;
                 if constexpr (FC == FMT_E2M1) {
                     uint32_t q[4];
 #pragma unroll
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
             }
         }
         const int e8 = wire_e8<FC>(words_amax<FC>(w[h]));
-        s_cscale[c * 4 + rb] = (uint8_t)(127 - e8);
+        s_cscale[c * RB + rb] = (uint8_t)(127 - e8);
         if constexpr (Fmt<FC>::hw) {
             uint32_t q[8];
 #pragma unroll
@@ -490,10 +492,9 @@ __global__ __launch_bounds__(DT) void k_mx_dual(const uint4* in, uint8_t* row_pa
     }
     // scale bytes of the column blocks: RB per column and tile
     if (tid < TILE_C && c < cols_valid) {
-        const uint32_t sall = *reinterpret_cast<const uint32_t*>(&s_cscale[c * 4]);
+        const uint32_t sall = *reinterpret_cast<const uint32_t*>(&s_cscale[c * RB]);
         uint8_t* dst = col_scales + (C0 + c) * ((rows + 31) / 32) + R0 / 32;
-        if (RB == 4 && (rows & 127) == 0) *reinterpret_cast<uint32_t*>(dst) = sall;
-        else if (RB == 2 && (rows & 63) == 0) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)sall;
+        if ((rows & 127) == 0) *reinterpret_cast<uint32_t*>(dst) = sall;
         else
             for (int b = 0; b < (rows_valid + 31) / 32; ++b) dst[b] = (uint8_t)(sall >> (8 * b));
     }
@@ -838,7 +839,7 @@ static int launch_dual(const void* input, void* row_payload, void* row_scales, v
     // 41.7 us, E4M3 56.5 -> 52.3, E2M3 56.4 -> 51.7; in the last-level cache 33.6 -> 32.8, 42.0 -> 41.6, 41.5 -> 41.8; 16384 x
     // 14336 E2M1 167 -> 145, E4M3 197 -> 190; 8192 x 4096 E4M3 30.3 -> 29.6 and 21.7 -> 22.8.  Below, 4096 x 4096, 10.6 -> 11.9.
     const unsigned spare = rows * cols >= ((int64_t)1 << 25) ? 40000u : 0u;
-    k_mx_dual<FR, FC, TILE_ROWS, DUAL_THREADS><<<(unsigned)(tiles_y * tiles_x), DUAL_THREADS, spare, st>>>(
+    k_mx_dual<FR, FC><<<(unsigned)(tiles_y * tiles_x), DUAL_THREADS, spare, st>>>(
         static_cast<const uint4*>(input), static_cast<uint8_t*>(row_payload), static_cast<uint8_t*>(row_scales),
         static_cast<uint8_t*>(col_payload), static_cast<uint8_t*>(col_scales), rows, cols, dual_tile_map(tiles_x, tiles_y));
     return mor_check_launch("k_mx_dual");
