@@ -22,9 +22,12 @@ namespace mor {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi}); }
 
-// 1 / (1 + exp(-x)); exp and the reciprocal are the one-ulp instructions, far inside bf16's half step of 2^-9 of a value.
-// Below x = -87.3, where it is under 2^-126, it may come out as 0.
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x)); }
+// 1 / (1 + exp(-x)); exp and the reciprocal are the one-ulp instructions, far inside bf16's half step of 2^-8 of a value.
+// They give 0 for what is below 2^-126: the reciprocal is taken of a quarter of its argument, so that the product with 1/4
+// keeps a subnormal result as far down as exp(-x) is finite (x > -88.8).
+__device__ __forceinline__ float sigmoid(float x) {
+    return 0.25f * __builtin_amdgcn_rcpf(0.25f + __builtin_amdgcn_exp2f(__builtin_fmaf(-1.44269504f, x, -2.0f)));
+}
 
 struct SwigluShape {
     int64_t rows, cols;
