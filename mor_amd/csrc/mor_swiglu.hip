@@ -6,9 +6,9 @@
 // Forward reads 4 and writes 2 + 2.0625 bytes per element, backward reads 2 + 2.0625 and writes 4.  A lane owns 8
 // consecutive elements of a row, a quad of lanes a block (k_swiglu_mx / k_swiglu_mx_backward); arithmetic in fp32, one
 // rounding to bf16 per result (bf16 is the tensors' type), the codes' rounding is the E4M3 grid's.
-// Bound by memory: 16384 x 14336 takes 306 us either way, 6.2 TB/s (a 2 GiB copy reaches 4.9, a cold one of 128 MiB 6.2).  Rows that cannot be
-// read as aligned vectors go element by element, which the caches gather: 4096 x 14335 87 us, x 14336 82; whole chunks as
-// one access at a 2-byte address are no faster (86).
+// Bound by memory: 16384 x 14336 takes 306 us forward and 286 backward, 6.2 and 6.6 TB/s (a 2 GiB copy reaches 4.9, a cold one
+// of 128 MiB 6.2).  Rows that cannot be read as aligned vectors go element by element, at two to three times the time: 4096 x
+// 14335 195 us forward and 231 backward, x 14336 84 and 75.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
