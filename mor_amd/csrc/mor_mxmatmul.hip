@@ -55,15 +55,20 @@ static int bits_of(int fmt) { return fmt == MOR_FMT_E2M1 ? 4 : 8; }
 //
 // Tiles of 128 or 64 and the parts that k is split into: 4 us, and a time per step that grows where two workgroups share a
 // CU's copies, but no less than the operands at 5 TB/s; for a split k 3 us more and 8 bytes per result and part at 4 TB/s.
-//   E4M3                      T = 64: whole, split     T = 128, eight waves     T = 128, four waves: whole, split
-//   1000 x 1000 x 1024             4.7, 10.8 in 2             7.3                       8.1
-//   512 x 4096 x 4096             16.9                       20.4                      23.5
-//   1024 x 4096 x 4096            30.6                       22.2                      25.7
-//   64 x 4096 x 4096              12.5, 10.0 in 4            19.0                      22.4, 12.5 in 4
-//   128 x 4096 x 14336            38.4, 20.6 in 4            64.1                      75.1, 22.8 in 8
-//   700 x 1000 x 14336            38.9, 29.8 in 2            64.0                      26.6 in 8
-//   64 x 65536 x 4096             66.7                                                 68.6              (T = 256: 85.1)
-//   128 x 65536 x 4096            94.7                                                 69.8              (T = 256: 84.2)
+// T = 64 whole | in parts (how many), T = 128 in eight waves, T = 128 in four | in parts:
+//                             E4M3                                  E4M3 x E2M1                          E2M1
+//   1000 x 1000 x 1024         4.7, 7.2, 7.4                         4.4, 6.6, 6.9                        4.2, 5.2, 5.3
+//   256 x 4096 x 4096         13.4 | 15.8 (2), 20.0, 22.9            11.9 | 15.2 (2), 17.4, 20.4          10.6 | 14.2 (2), 14.4, 13.4
+//   512 x 4096 x 4096         16.5, 20.3, 23.4 | 21.9 (2)            14.2, 17.7, 20.8 | 21.4 (2)          11.9, 14.6, 13.8 | 20.9 (2)
+//   1024 x 4096 x 4096        30.7, 22.3, 25.6                       25.8, 19.7, 22.5                     18.1, 16.3, 15.9
+//   2048 x 4096 x 4096        61.2, 42.9, 34.4                       49.5, 37.7, 32.1                     34.0, 23.8, 23.1
+//   64 x 4096 x 4096          12.4 | 10.0 (4), 18.9, 22.2 | 12.5     10.8 | 9.2 (4), 15.4, 18.9 | 11.7    7.7 | 8.9 (4), 10.9, 10.8 | 10.0
+//   128 x 4096 x 14336        38.0 | 20.7 (4), 63.8, 74.9 | 22.9 (8) 32.9 | 17.9 (4), 54.6, 67.0 | 21.2   28.8 | 15.8 (4), 45.4, 40.4 | 16.7
+//   700 x 1000 x 14336        38.8 | 30.1 (2), 63.6, 72.5 | 26.5 (7) 33.5 | 25.4 (2), 56.0, 64.8 | 25.1   29.4 | 21.5 (2), 43.3, 39.1 | 19.2 (4)
+//   64 x 65536 x 4096         68.0, 74.5, 69.1                       44.9, 49.0, 40.6                     37.4, 36.0, 34.2
+//   128 x 65536 x 4096        97.0, 79.5, 72.6                       80.2, 57.2, 44.4                     56.7, 40.5, 37.1
+// A mixed pair is priced as an 8-bit one: its order is the same but for 64 x 65536 x 4096 (10 % lost).  Two 4-bit operands gain
+// nothing from eight waves that four, whose steps have 256 columns there too, do not give.
 // More tiles than run at once only where they are a single row or column: else the operands are read too often.
 static double small_tiles(MxPlan& q, int64_t m, int64_t n, int64_t k, int bits_a, int bits_b, bool split) {
     const bool both4 = bits_a == 4 && bits_b == 4;
