@@ -41,7 +41,7 @@ def _stream(x: Tensor) -> int:
 def quantize_mx(x: Tensor, fmt: int = E4M3) -> Tuple[Tensor, Tensor]:
     """-> (payload uint8 [rows, cols * bits / 8], scales uint8 [rows, cols / 32]); blocks of 32 along rows.  E2M1 has two
     codes to a byte, the first in the low half; a block with an infinity or a NaN has scale byte 255 there and decodes to
-    NaNs."""
+    NaNs.  E4M3 turns an infinity into a NaN, E5M2 keeps it."""
     return _op.mx_quantize(x, fmt)
 
 
@@ -61,7 +61,8 @@ def matmul_mx(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, a_fmt: i
     """a b^T of two tensors in the wire format -> bfloat16 [m, n]: payloads [m, k * bits / 8] and [n, k * bits / 8] and
     scales [m, k / 32] and [n, k / 32] as quantize_mx gives them.  Formats E4M3, E5M2 and E2M1 in any pair (b_fmt: that
     of a when not given).  The scaled matrix instructions read codes and scale bytes as they are, sum in fp32, and the
-    sum is rounded once; the same operands give the same bits.  A NaN in a row of a or b makes that row or column NaN."""
+    sum is rounded once; the same operands give the same bits.  A NaN in a row of a or b makes that row or column NaN; an infinity of
+    E5M2 counts as one."""
     return _op.mx_matmul(a, a_scales, b, b_scales, a_fmt, a_fmt if b_fmt is None else b_fmt)
 
 
