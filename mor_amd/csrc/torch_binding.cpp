@@ -279,9 +279,10 @@ std::tuple<at::Tensor, at::Tensor> swiglu_backward(const at::Tensor& grad, const
     const int64_t rows = d.size(0), cols = d.size(1);
     const SwigluKept k(rows, cols);
     TORCH_CHECK(kept.scalar_type() == at::kByte && kept.device() == d.device() && kept.is_contiguous() && kept.numel() == k.bytes, "mor: kept does not match grad");
+    const at::Tensor at16 = aligned(kept, 16);             // (a saved-tensor hook may bring it back anywhere)
     const c10::OptionalDeviceGuard guard(d.device());
     at::Tensor dg = at::empty({rows, cols}, d.options()), du = at::empty({rows, cols}, d.options());
-    const uint8_t* b = kept.data_ptr<uint8_t>();
+    const uint8_t* b = at16.data_ptr<uint8_t>();
     if (d.numel()) check(mor_swiglu_mx_backward(d.data_ptr(), b, b + 2 * k.codes, b + k.codes, b + 2 * k.codes + k.scales, dg.data_ptr(), du.data_ptr(), rows, cols, stream_of(d)));
     return {dg, du};
 }
@@ -363,6 +364,7 @@ std::tuple<at::Tensor, at::Tensor> linear_backward(const at::Tensor& grad, const
     const int64_t tokens = d.size(0), outputs = d.size(1), padded = cdiv(tokens, 32) * 32;
     const Kept k(tokens, inputs, outputs, fmt, kept_x, kept_w);
     TORCH_CHECK(kept.scalar_type() == at::kByte && kept.device() == d.device() && kept.is_contiguous() && kept.numel() == k.parts.bytes, "mor: kept does not match grad");
+    const at::Tensor at16 = aligned(kept, 16);             // (a saved-tensor hook may bring it back anywhere)
     const c10::OptionalDeviceGuard guard(d.device());
     const auto u8 = d.options().dtype(at::kByte);
     at::Tensor dx = at::empty({0}, d.options()), dw = dx;
@@ -376,8 +378,8 @@ std::tuple<at::Tensor, at::Tensor> linear_backward(const at::Tensor& grad, const
     const at::Tensor codes = at::empty({scratch.bytes}, u8);
     if (kept_x) quantize_into(d, grad_fmt, gr.of(codes), grad_fmt, gt.of(codes));
     else quantize_into(d, grad_fmt, gr.of(codes));
-    if (kept_w) dx = product(gr.of(codes), grad_fmt, k.wt.of(kept), fmt, tokens, inputs, outputs, u8, stream_of(d));
-    if (kept_x) dw = product(gt.of(codes), grad_fmt, k.xt.of(kept), MOR_FMT_E4M3, outputs, inputs, padded, u8, stream_of(d));
+    if (kept_w) dx = product(gr.of(codes), grad_fmt, k.wt.of(at16), fmt, tokens, inputs, outputs, u8, stream_of(d));
+    if (kept_x) dw = product(gt.of(codes), grad_fmt, k.xt.of(at16), MOR_FMT_E4M3, outputs, inputs, padded, u8, stream_of(d));
     return {dx, dw};
 }
 
