@@ -45,11 +45,12 @@ def quantize_mx(x: Tensor, fmt: int = E4M3) -> Tuple[Tensor, Tensor]:
     return _op.mx_quantize(x, fmt)
 
 
-def quantize_mx_dual(x: Tensor, fmt: int = E4M3) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+def quantize_mx_dual(x: Tensor, fmt: int = E4M3, col_fmt: Optional[int] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     """One read of x, both orientations: (payload, scales) of x as quantize_mx gives them and (payload, scales) of
-    x.t() -- the operands of the dgrad and wgrad GEMMs of a linear layer."""
-    _check(x, 32)
-    return _op.mx_quantize_dual(x, fmt, fmt)
+    x.t() -- the operands of the dgrad and wgrad GEMMs of a linear layer.  col_fmt: the format of x.t() where it is
+    another one; (E2M1, E4M3) is the pair there is.  In the 8- and 4-bit formats any number of rows: the last block of
+    each row of x.t() is filled up with zeros.  The 6-bit ones need a multiple of 32."""
+    return _op.mx_quantize_dual(x, fmt, fmt if col_fmt is None else col_fmt)
 
 
 def dequantize_mx(payload: Tensor, scales: Tensor, fmt: int = E4M3) -> Tensor:
