@@ -500,6 +500,19 @@ at::Tensor swiglu_autograd(const at::Tensor& gate, const at::Tensor& up) {
 // mor.ops.set_flavour: MOR_FLAG_* bits for every later call of the calling thread
 extern "C" __attribute__((visibility("default"))) void mor_torch_set_flags(uint32_t flags) { g_flags = flags; }
 
+static void mx_operators(torch::Library& m) {
+    m.impl("mx_quantize", &mx_quantize);
+    m.impl("mx_quantize_dual", &mx_quantize_dual);
+    m.impl("mx_dequantize", &mx_dequantize);
+    m.impl("mx_matmul", &mx_matmul);
+    m.impl("mx_linear", &mx_linear);
+    m.impl("mx_linear_forward", &linear_forward);
+    m.impl("mx_linear_backward", &linear_backward);
+    m.impl("swiglu_mx", &swiglu);
+    m.impl("swiglu_mx_forward", &swiglu_forward);
+    m.impl("swiglu_mx_backward", &swiglu_backward);
+}
+
 TORCH_LIBRARY_IMPL(mor, CUDA, m) {
     m.impl("fake_quantize", &fake_quantize);
     m.impl("fake_quantize_no_alloc", &fake_quantize_no_alloc);
@@ -521,17 +534,11 @@ TORCH_LIBRARY_IMPL(mor, CUDA, m) {
         return e8mx_impl(i, x, y, bx, by, q, s, nullptr); });
     m.impl("fake_quantize_e8mx_inplace", [](const at::Tensor& i, int64_t x, int64_t y, int64_t bx, int64_t by, int64_t q, int64_t s, at::Tensor result) {
         e8mx_impl(i, x, y, bx, by, q, s, &result); });
-    m.impl("mx_quantize", &mx_quantize);
-    m.impl("mx_quantize_dual", &mx_quantize_dual);
-    m.impl("mx_dequantize", &mx_dequantize);
-    m.impl("mx_matmul", &mx_matmul);
-    m.impl("mx_linear", &mx_linear);
-    m.impl("mx_linear_forward", &linear_forward);
-    m.impl("mx_linear_backward", &linear_backward);
-    m.impl("swiglu_mx", &swiglu);
-    m.impl("swiglu_mx_forward", &swiglu_forward);
-    m.impl("swiglu_mx_backward", &swiglu_backward);
+    mx_operators(m);
 }
+
+// (tensors in host memory: their checks refuse them by name)
+TORCH_LIBRARY_IMPL(mor, CPU, m) { mx_operators(m); }
 
 // autograd for the four differentiable forward ops; the in-place / no_alloc / test ops keep their Python registration
 TORCH_LIBRARY_IMPL(mor, Autograd, m) {
