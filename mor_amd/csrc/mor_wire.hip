@@ -364,10 +364,13 @@ __global__ __launch_bounds__(DUAL_THREADS) void k_mx_dual(const uint4* in, uint8
     const bool full = rows_valid == TR && cols_valid == TILE_C;            // the same in every lane
     uint4 v[NV];
     if (full) {
-        // (plain loads: past the caches an input that is still in the last-level cache takes longer, 8192 x 8192 E4M3 41.6 ->
-        // 47.1 us, E2M3 42.0 -> 48.5, and one that is not no less, 52.5 -> 53.6 and 51.7 -> 51.0)
-#pragma unroll
-        for (int k = 0; k < NV; ++k) v[k] = in[first + k * step];
+        // Inputs of 192 to 256 MiB, which fill the last-level cache by themselves, are read past the caches: written or read just
+        // before, 8192 x 14336 E4M3 takes 79 instead of 91 us (99.5 and 96 from memory), 16384 x 8192 90 and 103 (108 and 104),
+        // 12288 x 8192 67 and 72 (81 and 78).  Smaller ones stay there for the most part: 8192 x 8192 E4M3 47.1 us past the
+        // caches, 41.6 through them (53.6 and 52.5), E2M3 48.5 and 42.0 (51.0 and 51.7), 10240 x 8192 56.4 and 51.0 (63.5 and
+        // 62.7).  Of larger ones little does: 16384 x 14336 E4M3 205 and 193 (205 and 190), E2M3 178 and 186 (189 and 183).
+        const int64_t n = rows * cols;
+        load16_group(v, n >= ((int64_t)3 << 25) && n <= ((int64_t)1 << 27), [&](int k) { return in + first + k * step; });
     } else {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {

@@ -46,3 +46,20 @@ def test_refusals():
         wire.quantize_mx_dual(x[:, :48])
     with pytest.raises(RuntimeError, match="bfloat16"):
         wire.quantize_mx_dual(x.float())
+
+
+@pytest.mark.parametrize("shape", [(8192, 8192), (12301, 8192), (16384, 8192), (16416, 8192)], ids=str)
+@pytest.mark.parametrize("fmts", [(P.E4M3, None), (P.E2M1, P.E4M3)], ids=str)
+def test_every_size_class_gives_the_bits_of_the_single_calls(shape, fmts):
+    """Inputs below 192 MiB, of 192 to 256 MiB (read past the caches) and beyond: the halves of the call against
+    quantize_mx on x and on x transposed, its rows filled up with zeros."""
+    from mor_amd import wire
+    rows, cols = shape
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    got = wire.quantize_mx_dual(x, *fmts)
+    want = wire.quantize_mx(x, fmts[0])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    high = -(-rows // 32) * 32
+    want = wire.quantize_mx(torch.nn.functional.pad(x.t(), (0, high - rows)).contiguous(), fmts[0] if fmts[1] is None else fmts[1])
+    assert torch.equal(got[2], want[0]) and torch.equal(got[3], want[1])
