@@ -255,7 +255,7 @@ __device__ __forceinline__ uint32_t gather_scales(uint32_t sb) {
 
 // ------------------------------------------------------------------------------------------------
 // blocks of 32 along rows; the tensor is a flat array of 16-byte chunks (cols % 32 == 0).  Bound by memory: 8192 x 8192 takes
-// 32.6 us in E4M3 (6.2 TB/s), 27 in E2M1 (6.3 TB/s)
+// 33 to 34 us in E4M3 (6.0 to 6.2 TB/s), 27 in E2M1 (6.3 TB/s)
 template <int F, int NV>
 __global__ __launch_bounds__(WWG) void k_mx_quantize(const uint4* in, uint8_t* payload, uint8_t* scales, int64_t nchunks) {
     const int64_t base = (int64_t)blockIdx.x * (NV * WWG) + threadIdx.x;
