@@ -107,3 +107,20 @@ def test_captured_and_replayed(shape, pair):
         want = wire.matmul_mx(*sets[i], *pair)
         torch.cuda.synchronize()
         assert torch.equal(out, want), i
+
+
+def test_more_small_tiles_than_2_to_the_22():
+    """20 rows on 2^28 + 17 columns of 512: 69 GB of codes, 2^22 + 1 tiles of 64.  Rows of B repeat with a period, so the
+    results do too; those of one period are held to the smaller product's."""
+    from mor_amd import wire
+    if torch.cuda.mem_get_info()[0] + torch.cuda.memory_reserved() < 120 << 30:
+        pytest.skip("needs 120 GB of device memory")
+    rng = np.random.default_rng(22)
+    m, n, k, period = 20, 2 ** 28 + 17, 512, 4099
+    (pa, sa), (pb, sb) = base.dev(*base.operand(rng, m, k, C4, 2)), base.dev(*base.operand(rng, period, k, C4, 2))
+    want = wire.matmul_mx(pa, sa, pb, sb, C4)
+    times = -(-n // period)
+    got = wire.matmul_mx(pa, sa, pb.repeat(times, 1)[:n], sb.repeat(times, 1)[:n], C4)
+    whole = n // period * period
+    for r in range(m):
+        assert (got[r, :whole].view(-1, period) == want[r]).all() and torch.equal(got[r, whole:], want[r, : n - whole]), r
